@@ -341,24 +341,29 @@ def _attend(state):
 
 
 # ---------------------------------------------------------------- 64 bits
+def _two64(n):
+    """2^n for whole n, exactly: a power function may be off in its last bit."""
+    return ((n.long() + 1023) << 52).view(torch.float64)
+
+
 def _grid64(x):
     """Rows x in 64 bits -> the values that the cache holds for them."""
     amax = x.abs().max(-1, keepdim=True).values
     e = torch.ceil(torch.log2(amax.clamp(min=1e-300) / 448.0))
-    e = e - (amax * 2.0 ** (1.0 - e) <= 448.0).double()          # the logarithm's own rounding
-    e = (e + (amax * 2.0 ** -e > 448.0).double()).clamp(-60.0, 60.0)
-    y = (x * 2.0 ** -e).clamp(-448.0, 448.0)
-    step = 2.0 ** (torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3.0)
-    return torch.round(y / step) * step * 2.0 ** e
+    e = e - (amax * _two64(1 - e) <= 448.0).double()             # the logarithm's own rounding
+    e = (e + (amax * _two64(-e) > 448.0).double()).clamp(-60.0, 60.0)
+    y = (x * _two64(-e)).clamp(-448.0, 448.0)
+    low = torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6)))
+    step = _two64(low - (_two64(low) > y.abs().clamp(min=2.0 ** -6)).double() - 3.0)
+    return torch.round(y / step) * step * _two64(e)
 
 
 def _held64(state, name, at):
     """Rows of the cache at `at` (page, offset) in 64 bits, [n, Hkv, D]."""
     c = state[name].view(torch.uint8)[at[0], :, at[1]].long()
     mant, ex = (c & 7).double(), (c >> 3) & 15
-    mag = torch.where(ex > 0, (1.0 + mant / 8.0) * 2.0 ** (ex.double() - 7.0), mant * 2.0 ** -9)
-    e = state[name + "_exp"][at[0], :, at[1]].double()
-    return torch.where(c > 127, -mag, mag) * (2.0 ** e)[..., None]
+    mag = torch.where(ex > 0, (1.0 + mant / 8.0) * _two64(ex - 7), mant * 2.0 ** -9)
+    return torch.where(c > 127, -mag, mag) * _two64(state[name + "_exp"][at[0], :, at[1]])[..., None]
 
 
 def exact(case, seed):
