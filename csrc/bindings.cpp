@@ -10,6 +10,8 @@
 
 #include "omni_kernels.h"
 
+void bind_kv8(pybind11::module_& m);   // bindings_kv8.cpp
+
 namespace {
 
 #define OMNI_CHECK_CUDA(t) TORCH_CHECK((t).is_cuda(), #t " must be a CUDA tensor")
@@ -916,4 +918,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("conv_transpose_ola", &conv_transpose_ola, "transposed-conv overlap-add + bias + causal trim");
   m.def("dwconv1d_causal", &dwconv1d_causal, "depthwise causal conv1d");
   m.def("conv2d_im2col", &conv2d_im2col, "2-D conv im2col rows (kh, kw, c)");
+  bind_kv8(m);
 }

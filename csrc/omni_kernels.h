@@ -180,6 +180,70 @@ struct RopeStoreArgs {
 };
 cudaError_t qkv_rope_store(const RopeStoreArgs& a, cudaStream_t stream);
 
+// ---------------------------------------------------------------- 8-bit paged KV cache (form: kv8.cuh)
+struct Kv8StoreArgs {
+  const void* qkv;         // [tokens, (hq + 2 hkv) * D] bf16, read only
+  int64_t qkv_stride;
+  int tokens, hq, hkv, head_dim;
+  void* q_out;             // [tokens, hq * D] bf16 rows of q_out_stride
+  int64_t q_out_stride;
+  const void* q_norm;      // [D] bf16 or nullptr
+  const void* k_norm;
+  float eps;
+  const int* positions;    // [pos_rows, tokens]; read when rot_dim > 0
+  int pos_rows;            // 1 (plain RoPE) or 3 (M-RoPE t/h/w)
+  int section[3];          // M-RoPE frequency sections (pairs)
+  int interleaved;
+  const float* cos_tab;    // [max_pos, rot_dim / 2]
+  const float* sin_tab;
+  int max_pos;             // positions are clamped into [0, max_pos)
+  int rot_dim;             // rotated dims (<= D); 0 disables RoPE
+  int neox;                // 1: rotate halves, 0: rotate adjacent pairs
+  const int* slot_mapping; // [tokens] page * 64 + offset; outside [0, num_slots): k / v not stored
+  void* k;                 // codes [pages, hkv, 64, D]
+  void* v;
+  void* k_exp;             // exponents [pages, hkv, 64]
+  void* v_exp;
+  int64_t num_slots;
+};
+cudaError_t kv8_store(const Kv8StoreArgs& a, cudaStream_t stream);
+
+struct Kv8ReadArgs {
+  const int* slots;        // [count]; outside [0, num_slots): zero rows
+  int count, hkv, head_dim;
+  const void* k;
+  const void* v;
+  const void* k_exp;
+  const void* v_exp;
+  int64_t num_slots;
+  void* k_out;             // [count, hkv, D] bf16
+  void* v_out;
+};
+cudaError_t kv8_read(const Kv8ReadArgs& a, cudaStream_t stream);
+
+struct Kv8AttnArgs {
+  const void* q;           // [q_rows, hq * D] bf16 rows of q_stride
+  int64_t q_stride;
+  int q_rows;              // tokens of the batch
+  const void* k;
+  const void* v;
+  const void* k_exp;
+  const void* v_exp;
+  int num_pages;           // block-table entries outside [0, num_pages) read page 0
+  const int* block_table;  // [batch, >= bt_pages] rows of bt_stride
+  int64_t bt_stride;
+  int bt_pages;            // a request sees at most bt_pages * 64 keys
+  const int* cu_q;         // [batch + 1] first query row of each request; nullptr: one row each (decode)
+  const int* kv_lens;      // [batch] keys of each request, its new tokens included
+  int batch, hq, hkv, head_dim;
+  float scale;
+  int window;              // > 0: a query sees its last `window` keys and the first `sinks` tokens
+  int sinks;
+  void* out;               // [q_rows, hq * D] bf16 rows of out_stride
+  int64_t out_stride;
+};
+cudaError_t kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream);
+
 struct MoeRouteArgs {
   const float* logits;     // [tokens, experts] router logits (fp32)
   int64_t logits_stride;

@@ -30,7 +30,7 @@ CUDA_FLAGS = [
 if os.environ.get("OMNI_DEVICE_CHECKS"):
     CUDA_FLAGS.append("-DOMNI_DEVICE_CHECKS=1")
 
-cuda_sources = sorted(glob.glob(os.path.join("csrc", "*.cu"))) + ["csrc/bindings.cpp"]
+cuda_sources = sorted(glob.glob(os.path.join("csrc", "*.cu"))) + ["csrc/bindings.cpp", "csrc/bindings_kv8.cpp"]
 runtime_sources = sorted(glob.glob(os.path.join("csrc", "runtime", "*.cpp")))
 
 ext_modules = [
