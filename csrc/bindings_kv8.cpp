@@ -10,16 +10,20 @@ namespace {
 
 using OptTensor = c10::optional<torch::Tensor>;
 
+// Messages are built from strings alone: streaming a number into a message ends the process where
+// the image's C++ runtime and torch's differ.
+std::string num(int64_t v) { return std::to_string(v); }
+
 bool aligned16(const torch::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 
 void check_on(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device(), ", got ", t.device());
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on the cache's CUDA device");
 }
 
 // Rows of a 2-D bf16 tensor that the kernels read or write 16 bytes at a time.
 void check_rows(const torch::Tensor& t, int64_t cols, const char* name) {
   TORCH_CHECK(t.dim() == 2 && t.scalar_type() == at::kBFloat16, name, " must be a 2-D bf16 tensor");
-  TORCH_CHECK(t.size(1) >= cols, name, " has ", t.size(1), " columns, needs ", cols);
+  TORCH_CHECK(t.size(1) >= cols, name, " has " + num(t.size(1)) + " columns, needs " + num(cols));
   TORCH_CHECK(t.stride(1) == 1 && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= cols)) && aligned16(t), name,
               " must have contiguous rows, 16-byte aligned");
 }
@@ -32,7 +36,7 @@ Cache check_cache(const torch::Tensor& k, const torch::Tensor& v, const torch::T
   TORCH_CHECK(k.is_cuda() && k.dim() == 4 && k.scalar_type() == at::kFloat8_e4m3fn && k.size(2) == 64,
               "cache.k must be a CUDA float8_e4m3fn tensor [pages, Hkv, 64, D]");
   Cache c{k.size(0), k.size(1), k.size(3)};
-  TORCH_CHECK(c.d == 64 || c.d == 128, "the 8-bit cache takes head dims 64 and 128, got ", c.d);
+  TORCH_CHECK(c.d == 64 || c.d == 128, "the 8-bit cache takes head dims 64 and 128, got " + num(c.d));
   TORCH_CHECK(c.pages >= 1 && c.hkv >= 1 && c.pages * c.hkv * 64 < (int64_t{1} << 31),
               "cache.k: pages * Hkv * 64 must be in [1, 2^31)");
   check_on(v, k, "cache.v");
@@ -73,7 +77,7 @@ torch::Tensor kv8_store(const torch::Tensor& qkv, const torch::Tensor& k, const 
   const at::cuda::CUDAGuard guard(k.device());
   omni::Kv8StoreArgs a{};
   a.slot_mapping = int_ptr(slots, k, "slot_mapping");
-  TORCH_CHECK(slots.numel() == T, "slot_mapping has ", slots.numel(), " entries for ", T, " tokens");
+  TORCH_CHECK(slots.numel() == T, "slot_mapping has " + num(slots.numel()) + " entries for " + num(T) + " tokens");
   TORCH_CHECK(rot_dim >= 0 && rot_dim % 2 == 0 && rot_dim <= head_dim, "rot_dim must be even and in [0, head_dim]");
   if (rot_dim > 0) {
     TORCH_CHECK(positions.has_value() && cos_tab.has_value() && sin_tab.has_value(),
@@ -103,7 +107,7 @@ torch::Tensor kv8_store(const torch::Tensor& qkv, const torch::Tensor& k, const 
   torch::Tensor q = q_out.has_value() ? *q_out : torch::empty({T, hq * head_dim}, qkv.options());
   check_on(q, k, "out");
   check_rows(q, hq * head_dim, "out");
-  TORCH_CHECK(q.size(0) == T, "out has ", q.size(0), " rows for ", T, " tokens");
+  TORCH_CHECK(q.size(0) == T, "out has " + num(q.size(0)) + " rows for " + num(T) + " tokens");
   a.qkv = qkv.data_ptr();
   a.qkv_stride = qkv.stride(0);
   a.tokens = static_cast<int>(T);
@@ -156,7 +160,8 @@ std::tuple<torch::Tensor, torch::Tensor> kv8_read(const torch::Tensor& k, const 
 torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
                             const torch::Tensor& k_exp, const torch::Tensor& v_exp, const torch::Tensor& block_table,
                             const OptTensor& cu_q, const torch::Tensor& kv_lens, int64_t hq, int64_t hkv,
-                            int64_t head_dim, double scale, int64_t window, int64_t sinks, const OptTensor& out_) {
+                            int64_t head_dim, double scale, int64_t window, int64_t sinks, const OptTensor& out_,
+                            const OptTensor& status) {
   const Cache c = check_cache(k, v, k_exp, v_exp);
   TORCH_CHECK(head_dim == c.d && hkv == c.hkv, "the head dim / KV heads do not match the cache");
   TORCH_CHECK(hq >= 1 && hq % hkv == 0, "num_heads must be a multiple of num_kv_heads");
@@ -178,12 +183,12 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
     a.cu_q = int_ptr(*cu_q, k, "cu_q");
     TORCH_CHECK(cu_q->numel() == B + 1, "cu_q needs one entry more than kv_lens");
   } else {
-    TORCH_CHECK(T == B, "decode takes one query row per request: ", T, " rows, ", B, " requests");
+    TORCH_CHECK(T == B, "decode takes one query row per request: " + num(T) + " rows, " + num(B) + " requests");
   }
   torch::Tensor out = out_.has_value() ? *out_ : torch::empty({T, hq * head_dim}, q.options());
   check_on(out, k, "out");
   check_rows(out, hq * head_dim, "out");
-  TORCH_CHECK(out.size(0) == T, "out has ", out.size(0), " rows for ", T, " query rows");
+  TORCH_CHECK(out.size(0) == T, "out has " + num(out.size(0)) + " rows for " + num(T) + " query rows");
   if (T == 0) return out;
   TORCH_CHECK(B > 0, "query rows without a request");
   a.q = q.data_ptr();
@@ -206,7 +211,21 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
   a.sinks = static_cast<int>(sinks);
   a.out = out.data_ptr();
   a.out_stride = out.stride(0);
-  check_launch(omni::kv8_attention(a, at::cuda::getCurrentCUDAStream()), "kv8_attention");
+  if (status.has_value()) {
+    check_on(*status, k, "status");
+    TORCH_CHECK(status->scalar_type() == at::kInt, "status must be int32");
+    a.status = status->data_ptr<int>();
+  }
+  if (!cu_q.has_value()) {
+    a.ctas = omni::kv8_decode_ctas(at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+    // scratch from the caching allocator, used on the current stream only
+    torch::Tensor scratch = torch::empty({omni::kv8_decode_scratch_floats(a.ctas, static_cast<int>(hq / hkv), a.head_dim)},
+                                         k.options().dtype(at::kFloat));
+    a.scratch = scratch.data_ptr<float>();
+    check_launch(omni::kv8_decode(a, at::cuda::getCurrentCUDAStream()), "kv8_decode_attention");
+    return out;
+  }
+  check_launch(omni::kv8_attention(a, at::cuda::getCurrentCUDAStream()), "kv8_prefill_attention");
   return out;
 }
 

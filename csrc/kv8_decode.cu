@@ -1,0 +1,647 @@
+// Decode attention over the 8-bit paged KV cache (form: kv8.cuh): one query token per request.
+//
+//   o = sum_j p_j v_j,   p = softmax_j(q . k_j * scale) over the visible keys j
+//
+// Bound by the cache's bytes (2 (D + 1) per key and KV head), so the design is a stream of 64-key
+// tiles (one page of one KV head: contiguous) through a deep shared-memory ring, and cheap work on
+// each tile:
+//
+// * Work split.  The visible tiles of all (request, KV head) pairs form one sequence; CTA c takes
+//   the tiles [c * per, (c + 1) * per) of it, per = ceil(tiles / CTAs), found on the device from
+//   kv_lens.  Every CTA streams the same number of tiles whatever the lengths are, and the launch
+//   does not depend on them (CUDA graphs).  A pair that lies in several CTAs leaves partial sums,
+//   which a second, dependent launch joins in a fixed order.
+// * A producer warp issues TMA loads (K and V tile swizzled, their exponents as bulk copies);
+//   four consumer warps take 16 keys of every tile each and keep their own running maximum, sum
+//   and output until the pair ends, so tiles need no barrier among the warps.
+// * Arithmetic on 16 keys: the codes go to fp16 (exact), S^T = K Q^T and O^T += V^T P by
+//   mma.m16n8k16 with the keys / dims as the 16 rows and the query heads of the KV head as the
+//   columns, so few heads waste few rows.  The contraction order inside a 16-dim chunk is free, and
+//   is chosen so that an ldmatrix register's 4 codes are exactly one lane's operand values.
+//   tcgen05 is not used: its 128-row tiles would be filled to 1/16 by 8 heads, and the time is the
+//   memory's either way.
+// * Scales.  Exponents never touch the codes.  With t_j = log2-score + ev_j (ev: V's exponent),
+//   w_j = 2^(t_j - m) is key j's weight on its integer-like codes, held in fp16 for the product;
+//   m is the running maximum of t (raised only when exceeded by 8), so what fp16 drops is below
+//   2^-31 of the largest contribution.  The softmax sum takes w_j * 2^-ev_j in fp32.
+//   q is scaled by a power of two to [2^9, 2^10) before it is rounded to fp16.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_runtime.h>
+
+#include <mutex>
+
+#include "host_util.h"
+#include "kv8.cuh"
+#include "omni_kernels.h"
+#include "sm100.cuh"
+
+namespace omni {
+namespace {
+
+using namespace kv8;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWarps = 4;                       // consumer warps
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr float kRaise = 8.f;                   // log2 units
+constexpr float kHead = 7.f;                    // weights are held times 2^7: below 2^15
+
+template <int D, int NT>
+struct Smem {
+  static constexpr int kStages = NT == 1 ? 5 : 4;   // two CTAs per SM in 227 KB
+  static constexpr int kTile = kPage * D;       // bytes of a K or V tile
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kExp = kStages * kStage;                 // exponents: [stage][2][64]
+  static constexpr int kRedStride = D + 4;                      // floats; conflict-free float2 stores
+  static constexpr int kRed = kExp + kStages * 2 * kPage;       // [warp][8 NT heads][D + 4]
+  static constexpr int kMl = kRed + kWarps * 8 * NT * kRedStride * 4;   // [warp][8 NT][2] (m, l)
+  static constexpr int kBars = kMl + kWarps * 8 * NT * 8;
+  static constexpr int kBytes = kBars + 16 * kStages + 16 + 1024;
+};
+
+struct Params {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  const uint8_t* k_exp;
+  const uint8_t* v_exp;
+  const int* block_table;
+  int64_t bt_stride;
+  int bt_pages, num_pages;
+  const int* kv_lens;
+  int batch, hq, hkv, group, head_groups;       // head_groups: column tiles of 8 NT heads per KV head
+  float scale;
+  int window, sinks;
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  float* part_o;                                // [2 CTAs][8 NT][D]
+  float* part_ml;                               // [2 CTAs][8 NT][2]
+  int ctas;
+  int* status;
+};
+
+// Visible keys of a request and the 64-key tiles that hold them.
+struct Span {
+  int kv, lo, sinks;      // keys [0, sinks) and [lo, kv)
+  int sink_tiles, first, tiles;
+  __device__ Span(const Params& p, int b) {
+    kv = min(p.kv_lens[b], p.bt_pages * kPage);
+    lo = p.window > 0 ? max(0, kv - p.window) : 0;
+    sinks = min(p.sinks, lo);
+    first = lo >> 6;
+    sink_tiles = min((sinks + 63) >> 6, first);
+    tiles = kv > 0 ? sink_tiles + ((kv + 63) >> 6) - first : 0;
+  }
+  __device__ int tile(int i) const { return i < sink_tiles ? i : first + i - sink_tiles; }
+};
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// Tiles of all requests, and of those before request `stop` (whole warp).
+__device__ __forceinline__ int64_t count_tiles(const Params& p, int stop, int64_t* before) {
+  const int lane = threadIdx.x & 31;
+  int64_t all = 0, head = 0;
+  for (int b = lane; b < p.batch; b += 32) {
+    const int n = Span(p, b).tiles;
+    all += n;
+    if (b < stop) head += n;
+  }
+  if (before != nullptr) *before = warp_sum64(head);
+  return warp_sum64(all);
+}
+
+// Walks a CTA's tiles pair by pair (whole warp; every warp of the CTA walks alike).
+struct Walk {
+  int b, r;               // request; KV head * head_groups + head group
+  int i0, i1, n;          // this segment's tiles [i0, i1) of the pair's n
+  int64_t left;
+  int per_b;              // pairs per request
+  __device__ Walk(const Params& p, int64_t x0, int64_t x1, int R) {
+    per_b = R;
+    left = x1 - x0;
+    const int lane = threadIdx.x & 31;
+    int64_t cum = 0;
+    b = 0;
+    for (int base = 0; base < p.batch; base += 32) {
+      const int mine = base + lane < p.batch ? Span(p, base + lane).tiles : 0;
+      int64_t inc = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += up;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, (cum + inc) * R > x0);
+      if (past != 0) {
+        const int at = __ffs(past) - 1;
+        b = base + at;
+        n = __shfl_sync(0xffffffffu, mine, at);
+        cum += __shfl_sync(0xffffffffu, inc - mine, at);
+        break;
+      }
+      cum += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    const int64_t rel = x0 - cum * R;
+    r = static_cast<int>(rel / n);
+    i0 = static_cast<int>(rel - static_cast<int64_t>(r) * n);
+    i1 = static_cast<int>(min(static_cast<int64_t>(n), i0 + left));
+  }
+  __device__ bool next(const Params& p) {
+    left -= i1 - i0;
+    if (left <= 0) return false;
+    if (++r == per_b) {
+      r = 0;
+      do {
+        ++b;
+        n = Span(p, b).tiles;
+      } while (n == 0);
+    }
+    i0 = 0;
+    i1 = static_cast<int>(min(static_cast<int64_t>(n), left));
+    return true;
+  }
+};
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ uint32_t movm_t(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Byte offset of 16-byte chunk c of row r in a swizzled tile (128-byte swizzle for 128-byte rows,
+// 64-byte swizzle for 64-byte rows).
+template <int D>
+__device__ __forceinline__ int swz(int r, int c) {
+  return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads, 2)
+    kv8_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Params p) {
+  using S = Smem<D, NT>;
+  constexpr int kStages = S::kStages;
+  constexpr int C = D / 16;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  float* red = reinterpret_cast<float*>(smem + S::kRed);
+  float2* ml = reinterpret_cast<float2*>(smem + S::kMl);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* empty = full + kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  __syncthreads();
+  grid_dep_launch();   // the joining launch may set up; it waits for this grid before it reads
+
+  const int R = p.hkv * p.head_groups;
+  const int64_t W = count_tiles(p, 0, nullptr) * R;
+  const int64_t per = (W + p.ctas - 1) / p.ctas;
+  const int64_t x0 = blockIdx.x * per, x1 = min(W, x0 + per);
+  if (x0 >= x1) return;
+  Walk w(p, x0, x1, R);
+
+  if (warp == kWarps) {
+    // ------------------------------------------------------------ producer
+    int64_t t = 0;
+    bool ok = true;
+    do {
+      const Span sp(p, w.b);
+      const int h = w.r / p.head_groups;
+      const int* row = p.block_table + static_cast<int64_t>(w.b) * p.bt_stride;
+      for (int i = w.i0; i < w.i1 && ok; i += 32) {
+        const int mine = i + lane < w.i1 ? checked_page(row[sp.tile(i + lane)], p.num_pages) : 0;
+        const int m = min(32, w.i1 - i);
+        for (int j = 0; j < m; ++j, ++t) {
+          const int page = __shfl_sync(0xffffffffu, mine, j);
+          const int s = static_cast<int>(t % kStages);
+          bool go = true;
+          if (lane == 0) {
+            if (t >= kStages) go = mbar_wait(&empty[s], static_cast<uint32_t>((t / kStages) & 1) ^ 1u, abort_flag, p.status);
+            if (go) {
+              const int r0 = (page * p.hkv + h) * kPage;
+              uint8_t* dst = smem + s * S::kStage;
+              uint8_t* de = smem + S::kExp + s * 2 * kPage;
+              mbar_arrive_expect_tx(&full[s], S::kStage + 2 * kPage);
+              tma_load_2d(dst, &tk, &full[s], 0, r0);
+              bulk_copy(de, p.k_exp + r0, kPage, &full[s]);
+              tma_load_2d(dst + S::kTile, &tv, &full[s], 0, r0);
+              bulk_copy(de + kPage, p.v_exp + r0, kPage, &full[s]);
+            }
+          }
+          go = __shfl_sync(0xffffffffu, go, 0);
+          if (!go) {
+            ok = false;
+            break;
+          }
+        }
+      }
+    } while (ok && w.next(p));
+    // every issued load has landed before the CTA's shared memory goes away
+    if (lane == 0)
+      for (int64_t j = t > kStages ? t - kStages : 0; j < t; ++j)
+        mbar_wait(&full[j % kStages], static_cast<uint32_t>((j / kStages) & 1), nullptr, p.status);
+    return;
+  }
+
+  // -------------------------------------------------------------- consumers
+  const int g = lane >> 2, t4 = lane & 3;
+  const int lrow = warp * 16 + (lane & 15);                 // ldmatrix row of this lane
+  int64_t t = 0;
+  bool ok = true;
+  bool more = true;
+  while (more) {
+    const Span sp(p, w.b);
+    const int h = w.r / p.head_groups, hg = w.r - h * p.head_groups;
+    const int head0 = h * p.group + hg * 8 * NT;            // first query head of this pair
+    const int heads = min(8 * NT, p.group - hg * 8 * NT);
+    // Q fragments: lane (g, t4) holds dims 16 c + 4 t4 .. + 3 of head g (and g + 8)
+    uint32_t qf[NT][C][2];
+    float qs[NT][2];                                        // score factor of heads 2 t4, 2 t4 + 1
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float2 v[C][2];
+      uint32_t top = 0;
+      const bool live = nt * 8 + g < heads;
+      const __nv_bfloat16* qr = p.q + static_cast<int64_t>(w.b) * p.q_stride + static_cast<int64_t>(head0 + (live ? nt * 8 + g : 0)) * D + 4 * t4;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const uint2 two = live ? *reinterpret_cast<const uint2*>(qr + 16 * c) : make_uint2(0u, 0u);
+        v[c][0] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two.x));
+        v[c][1] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two.y));
+        top = max(max(top, __float_as_uint(v[c][0].x) & 0x7fffffffu), __float_as_uint(v[c][0].y) & 0x7fffffffu);
+        top = max(max(top, __float_as_uint(v[c][1].x) & 0x7fffffffu), __float_as_uint(v[c][1].y) & 0x7fffffffu);
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool bad = top >= 0x7f800000u;                  // inf / NaN in q: its output is NaN
+      const int x = max(static_cast<int>(top >> 23) - 127, -110);
+      const float up = bad ? 0.f : __int_as_float((9 - x + 127) << 23);
+      const float f = bad ? __int_as_float(0x7fc00000) : __int_as_float((x - 9 + 127) << 23) * p.scale * kLog2e;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) qf[nt][c][i] = bad ? 0u : pack_h2(v[c][i].x * up, v[c][i].y * up);
+      qs[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t4);
+      qs[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
+    }
+    float o[NT][C][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][c][i] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+
+    for (int i = w.i0; i < w.i1; ++i, ++t) {
+      const int s = static_cast<int>(t % kStages);
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], static_cast<uint32_t>((t / kStages) & 1), abort_flag, p.status));
+      if (!ok) continue;
+      const uint32_t kt = smem_u32(smem + s * S::kStage), vt = kt + S::kTile;
+      const int8_t* ex = reinterpret_cast<const int8_t*>(smem + S::kExp + s * 2 * kPage) + warp * 16;
+      const int key0 = sp.tile(i) * kPage;
+      const bool edge = key0 + kPage > sp.kv || (key0 < sp.lo && key0 + kPage > sp.sinks);
+
+      // S^T: 16 keys x 8 NT heads
+      float sc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; c += 2) {
+        uint32_t r[4];
+        ldsm4(kt + swz<D>(lrow, c + (lane >> 4)), r);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t a0 = e4m3x2_to_f16x2(r[2 * u]), a2 = e4m3x2_to_f16x2(r[2 * u] >> 16);
+          const uint32_t a1 = e4m3x2_to_f16x2(r[2 * u + 1]), a3 = e4m3x2_to_f16x2(r[2 * u + 1] >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma(sc[nt], a0, a1, a2, a3, qf[nt][c + u][0], qf[nt][c + u][1]);
+        }
+      }
+      // weights
+      float kf[2], ve[2], vi[2];
+      bool vis[2] = {true, true};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int j = g + 8 * u;
+        const int ev = ex[kPage + j];
+        const int ec = max(kExpMin, min(kExpMax, ev));
+        kf[u] = pow2_of(ex[j]);
+        ve[u] = ev == kExpBad ? __int_as_float(0x7fc00000) : static_cast<float>(ec);
+        vi[u] = __int_as_float((127 - ec) << 23);
+        if (edge) {
+          const int key = key0 + warp * 16 + j;
+          vis[u] = key < sp.kv && (key >= sp.lo || key < sp.sinks);
+        }
+      }
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            x[2 * u + v] = fmaf(sc[nt][2 * u + v], qs[nt][v] * kf[u], ve[u]);
+            if (!vis[u]) x[2 * u + v] = -INFINITY;
+          }
+        const bool grow = x[0] > m[nt][0] + kRaise || x[2] > m[nt][0] + kRaise || x[1] > m[nt][1] + kRaise || x[3] > m[nt][1] + kRaise;
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            float mx = fmaxf(x[v], x[2 + v]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float mn = fmaxf(m[nt][v], mx);
+            const float f = m[nt][v] == -INFINITY ? 0.f : ex2(m[nt][v] - mn);
+            m[nt][v] = mn;
+            l[nt][v] *= f;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              o[nt][c][v] *= f;
+              o[nt][c][2 + v] *= f;
+            }
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const float sub = m[nt][v] == -INFINITY ? 0.f : m[nt][v] - kHead;
+          x[v] = ex2(x[v] - sub);
+          x[2 + v] = ex2(x[2 + v] - sub);
+          l[nt][v] += x[v] * vi[0] + x[2 + v] * vi[1];
+        }
+        pb[nt][0] = movm_t(pack_h2(x[0], x[1]));
+        pb[nt][1] = movm_t(pack_h2(x[2], x[3]));
+      }
+      // O^T += V^T P; keys outside the visible range may hold anything: their codes become zeros
+      uint32_t keep[2] = {~0u, ~0u};
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int key = key0 + warp * 16 + 8 * u + 2 * t4;
+          const bool a = key < sp.kv && (key >= sp.lo || key < sp.sinks);
+          const bool b = key + 1 < sp.kv && (key + 1 >= sp.lo || key + 1 < sp.sinks);
+          keep[u] = (a ? 0xffffu : 0u) | (b ? 0xffff0000u : 0u);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < C; c += 2) {
+        uint32_t r[4];
+        ldsm4_t(vt + swz<D>(lrow, c + (lane >> 4)), r);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          // bytes (key 2t: dims 2g, 2g+1; key 2t+1: the same) -> two keys of a dim side by side
+          const uint32_t lo = __byte_perm(r[2 * u] & keep[0], 0u, 0x3120), hi = __byte_perm(r[2 * u + 1] & keep[1], 0u, 0x3120);
+          const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(lo >> 16);
+          const uint32_t a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma(o[nt][c + u], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+    }
+
+    // join the four warps
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        float x = l[nt][v];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int head = nt * 8 + 2 * t4 + v;
+        if (g == 0) ml[warp * 8 * NT + head] = make_float2(m[nt][v], x);
+        float* dst = red + (warp * 8 * NT + head) * S::kRedStride + 2 * g;
+#pragma unroll
+        for (int c = 0; c < C; ++c) *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[nt][c][v], o[nt][c][2 + v]);
+      }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const bool whole = w.i0 == 0 && w.i1 == w.n;
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (w.i0 == 0 ? 1 : 0);
+    for (int e = threadIdx.x; e < heads * (D / 4); e += 32 * kWarps) {
+      const int head = e / (D / 4), d = (e - head * (D / 4)) * 4;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kWarps; ++u) mm = fmaxf(mm, ml[u * 8 * NT + head].x);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float ll = 0.f;
+#pragma unroll
+      for (int u = 0; u < kWarps; ++u) {
+        const float2 v = ml[u * 8 * NT + head];
+        // a warp without a finite maximum has either nothing (0) or a NaN to pass on
+        const float f = v.x == -INFINITY ? 1.f : ex2(v.x - mm);
+        const float4 x = *reinterpret_cast<const float4*>(red + (u * 8 * NT + head) * S::kRedStride + d);
+        acc.x += x.x * f;
+        acc.y += x.y * f;
+        acc.z += x.z * f;
+        acc.w += x.w * f;
+        ll += v.y * f;
+      }
+      if (whole) {
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        uint2 two;
+        __nv_bfloat162 y = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+        two.x = *reinterpret_cast<uint32_t*>(&y);
+        y = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+        two.y = *reinterpret_cast<uint32_t*>(&y);
+        *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(w.b) * p.out_stride + static_cast<int64_t>(head0 + head) * D + d) = two;
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + (slot * 8 * NT + head) * D + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * 8 * NT + head) * 2) = make_float2(mm, ll);
+      }
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    more = w.next(p);
+  }
+}
+
+// Joins the partial sums of split pairs in the order of their CTAs, and writes zeros for requests
+// without a visible key.  One warp per (request, query head).
+template <int D, int NT>
+__global__ void __launch_bounds__(128) kv8_decode_join_kernel(const Params p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp;
+  if (row >= static_cast<int64_t>(p.batch) * p.hq) {
+    grid_dep_wait();
+    return;
+  }
+  const int b = static_cast<int>(row / p.hq), hq = static_cast<int>(row - static_cast<int64_t>(b) * p.hq);
+  const int h = hq / p.group, in = hq - h * p.group, hg = in / (8 * NT), head = in - hg * 8 * NT;
+  const int R = p.hkv * p.head_groups;
+  int64_t before;
+  const int64_t W = count_tiles(p, b, &before) * R;
+  const int n = Span(p, b).tiles;
+  grid_dep_wait();                            // in every thread: what follows on the stream relies on it
+  constexpr int PER = D / 32;
+  __nv_bfloat16* out = p.out + static_cast<int64_t>(b) * p.out_stride + static_cast<int64_t>(hq) * D + lane * PER;
+  float acc[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+  float ll = 0.f;
+  if (n > 0) {
+    const int64_t per = (W + p.ctas - 1) / p.ctas;
+    const int64_t x = before * R + static_cast<int64_t>(h * p.head_groups + hg) * n;
+    const int64_t c0 = x / per, c1 = (x + n - 1) / per;
+    if (c0 == c1) return;                     // written by its CTA
+    auto slot = [&](int64_t c) { return (c == c0 ? 2 * c + 1 : 2 * c) * 8 * NT + head; };
+    float mm = -INFINITY;
+    for (int64_t c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, p.part_ml[slot(c) * 2]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+#pragma unroll 4
+    for (int64_t c = c0; c <= c1; ++c) {
+      const float2 v = *reinterpret_cast<const float2*>(p.part_ml + slot(c) * 2);
+      const float f = v.x == -INFINITY ? 1.f : ex2(v.x - mm);
+      const float* src = p.part_o + slot(c) * D + lane * PER;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] += src[i] * f;
+      ll += v.y * f;
+    }
+  }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll
+  for (int i = 0; i < PER; i += 2)
+    *reinterpret_cast<__nv_bfloat162*>(out + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+
+// Codes of one layer as [pages * Hkv * 64, D] bytes, box one page of one head.
+bool encode(CUtensorMap* map, const void* base, int d, int64_t rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(d)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(d), kPage};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, int NT>
+cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, cudaStream_t stream) {
+  using S = Smem<D, NT>;
+  cudaError_t e = ensure_smem_attr<kv8_decode_kernel<D, NT>>(S::kBytes);
+  if (e != cudaSuccess) return e;
+  kv8_decode_kernel<D, NT><<<p.ctas, kThreads, S::kBytes, stream>>>(tk, tv, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.batch) * p.hq + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv8_decode_join_kernel<D, NT>, p);
+}
+
+}  // namespace
+
+int kv8_decode_ctas(int sm_count) { return 2 * sm_count; }
+
+int64_t kv8_decode_scratch_floats(int ctas, int group, int head_dim) {
+  return 2 * static_cast<int64_t>(ctas) * (group > 8 ? 16 : 8) * (head_dim + 2);
+}
+
+cudaError_t kv8_decode(const Kv8AttnArgs& a, cudaStream_t stream) {
+  if (a.batch == 0) return cudaSuccess;
+  CUtensorMap tk, tv;
+  const int64_t rows = static_cast<int64_t>(a.num_pages) * a.hkv * kPage;
+  if (!encode(&tk, a.k, a.head_dim, rows) || !encode(&tv, a.v, a.head_dim, rows)) return cudaErrorInvalidValue;
+  Params p{};
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.q_stride = a.q_stride;
+  p.k_exp = static_cast<const uint8_t*>(a.k_exp);
+  p.v_exp = static_cast<const uint8_t*>(a.v_exp);
+  p.block_table = a.block_table;
+  p.bt_stride = a.bt_stride;
+  p.bt_pages = a.bt_pages;
+  p.num_pages = a.num_pages;
+  p.kv_lens = a.kv_lens;
+  p.batch = a.batch;
+  p.hq = a.hq;
+  p.hkv = a.hkv;
+  p.group = a.hq / a.hkv;
+  const int nt = p.group > 8 ? 2 : 1;
+  p.head_groups = (p.group + 8 * nt - 1) / (8 * nt);
+  p.scale = a.scale;
+  p.window = a.window;
+  p.sinks = a.sinks;
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.out_stride = a.out_stride;
+  p.ctas = a.ctas;
+  p.part_o = a.scratch;
+  p.part_ml = a.scratch + 2 * static_cast<int64_t>(a.ctas) * 8 * nt * a.head_dim;
+  p.status = a.status;
+  if (a.head_dim == 128) return nt == 1 ? launch<128, 1>(tk, tv, p, stream) : launch<128, 2>(tk, tv, p, stream);
+  if (a.head_dim == 64) return nt == 1 ? launch<64, 1>(tk, tv, p, stream) : launch<64, 2>(tk, tv, p, stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace omni

@@ -21,7 +21,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _check
-from ._ext import ext
+from ._ext import ext, status_word
 from .rope import apply_rope_ref
 
 PAGE = 64
@@ -170,7 +170,8 @@ def kv8_decode_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Te
         if _check.enabled():
             _check.check_paged("kv8_decode_attention", block_table, kv_lens, cache.k.shape[0])
         return ext().kv8_attention(q, cache.k, cache.v, cache.k_exp, cache.v_exp, block_table, None, kv_lens,
-                                   num_heads, num_kv_heads, head_dim, scale, window, sinks, out)
+                                   num_heads, num_kv_heads, head_dim, scale, window, sinks, out,
+                                   status_word(q.device))
     return _attention_cpu(q, cache, block_table, [1] * kv_lens.shape[0], kv_lens, num_heads, num_kv_heads, head_dim,
                           scale, window, sinks, out)
 
@@ -186,7 +187,8 @@ def kv8_prefill_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.T
         if _check.enabled():
             _check.check_paged("kv8_prefill_attention", block_table, kv_lens, cache.k.shape[0], cu_q, q.shape[0])
         return ext().kv8_attention(q, cache.k, cache.v, cache.k_exp, cache.v_exp, block_table, cu_q, kv_lens,
-                                   num_heads, num_kv_heads, head_dim, scale, window, sinks, out)
+                                   num_heads, num_kv_heads, head_dim, scale, window, sinks, out,
+                                   status_word(q.device))
     cu = cu_q.tolist()
     return _attention_cpu(q, cache, block_table, [b - a for a, b in zip(cu, cu[1:])], kv_lens, num_heads, num_kv_heads,
                           head_dim, scale, window, sinks, out)

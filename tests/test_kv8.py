@@ -176,7 +176,7 @@ def test_store(d, hq, hkv, rope, norm, tokens):
     assert torch.equal(c.v_exp[s // PAGE, :, s % PAGE].long(), e)
     got = K._rows_ref(c, s)
     assert torch.equal(got[1].double(), v)                    # V comes in as bf16: exact
-    k = prep(x[live][:, hq:hq + hkv], kn)
+    k = prep(x[:, hq:hq + hkv], kn)[live]
     if not norm and not rot:
         assert torch.equal(got[0].double(), hold64(k)[0])
     else:
