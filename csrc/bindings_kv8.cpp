@@ -1,4 +1,4 @@
-// torch bindings of the 8-bit paged KV cache (kv8_cache.cu, kv8_attention.cu).  Every argument is
+// torch bindings of the 8-bit paged KV cache (kv8_cache.cu, kv8_decode.cu, kv8_prefill.cu).  Every argument is
 // checked here, before anything is launched; a bad one raises with its name.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -165,6 +165,8 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
   const Cache c = check_cache(k, v, k_exp, v_exp);
   TORCH_CHECK(head_dim == c.d && hkv == c.hkv, "the head dim / KV heads do not match the cache");
   TORCH_CHECK(hq >= 1 && hq % hkv == 0, "num_heads must be a multiple of num_kv_heads");
+  TORCH_CHECK(hq / hkv <= 128, "at most 128 query heads per KV head");
+  TORCH_CHECK(scale > 0 && scale < 1e30, "scale must be positive");
   TORCH_CHECK(window >= 0 && sinks >= 0 && window < (int64_t{1} << 31) && sinks < (int64_t{1} << 31),
               "window and sinks must not be negative");
   check_on(q, k, "q");
@@ -216,16 +218,23 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
     TORCH_CHECK(status->scalar_type() == at::kInt, "status must be int32");
     a.status = status->data_ptr<int>();
   }
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  // scratch from the caching allocator, used on the current stream only
+  const auto f32 = k.options().dtype(at::kFloat);
+  torch::Tensor scratch;
   if (!cu_q.has_value()) {
-    a.ctas = omni::kv8_decode_ctas(at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
-    // scratch from the caching allocator, used on the current stream only
-    torch::Tensor scratch = torch::empty({omni::kv8_decode_scratch_floats(a.ctas, static_cast<int>(hq / hkv), a.head_dim)},
-                                         k.options().dtype(at::kFloat));
+    a.ctas = omni::kv8_decode_ctas(sms);
+    scratch = torch::empty({omni::kv8_decode_scratch_floats(a.ctas, static_cast<int>(hq / hkv), a.head_dim)}, f32);
     a.scratch = scratch.data_ptr<float>();
     check_launch(omni::kv8_decode(a, at::cuda::getCurrentCUDAStream()), "kv8_decode_attention");
-    return out;
+  } else {
+    a.splits = omni::kv8_prefill_splits(a, sms);
+    if (a.splits > 1) {
+      scratch = torch::empty({omni::kv8_prefill_scratch_floats(a)}, f32);
+      a.scratch = scratch.data_ptr<float>();
+    }
+    check_launch(omni::kv8_prefill(a, at::cuda::getCurrentCUDAStream()), "kv8_prefill_attention");
   }
-  check_launch(omni::kv8_attention(a, at::cuda::getCurrentCUDAStream()), "kv8_prefill_attention");
   return out;
 }
 

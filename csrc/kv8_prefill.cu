@@ -1,0 +1,662 @@
+// Chunk attention over the 8-bit paged KV cache (form: kv8.cuh) on the 5th-generation tensor cores.
+//
+//   o_i = sum_j p_ij v_j,   p_i = softmax_j(q_i . k_j * scale) over the keys j visible to query i
+//
+// Bound by the tensor cores (4 D operations per visible pair) for long chunks, by the softmax's
+// exponentials next, and by the cache's bytes when a chunk has few rows.
+//
+// One CTA: two 128-row query tiles (GQA-packed: row r = token tok0 + r / G, head h G + r % G) that
+// share every 64-key block (one page), and a range of the blocks they see:
+//
+// * Loader warps (4) read a block's codes and exponents into registers one block ahead, turn them
+//   into bf16 (exact: 4 significant bits times a power of two) and store them in the swizzled layout
+//   the tensor cores read; the cache's bytes cross HBM once per CTA at half of bf16's.
+// * One warp issues S = Q K^T and O += P V with S, P and O in tensor memory.  S has two buffers per
+//   tile: S of block j + 2 is issued once PV of block j is done, so the softmax never waits for the
+//   tensor core's latency, and P (bf16) takes the place of its S, so it never goes through shared memory.
+// * Two softmax warpgroups, one thread per row: running maximum (raised only when exceeded by 2^8),
+//   32-bit sums, O rescaled in tensor memory when the maximum is raised.
+//
+// Chunks with few row tiles split the key blocks over the grid's third dimension; the partial
+// outputs are joined in order by a second, dependent launch.  The row tiles are found on the device
+// from cu_q, so a launch depends on sizes alone.
+//
+// A key whose K or V row is marked as not finite enters as a NaN key row and a zero value row: its
+// scores are NaN for the queries that see it, and masked by selection for those that do not.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "host_util.h"
+#include "kv8.cuh"
+#include "omni_kernels.h"
+#include "sm100.cuh"
+
+namespace omni {
+namespace {
+
+using namespace kv8;
+
+constexpr int kRows = 128;                 // rows of a query tile
+constexpr int kBN = kPage;                 // keys of a block
+constexpr int kStages = 5;
+constexpr int kLoaders = 128;
+constexpr int kThreads = 256 + kLoaders + 32;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaise = 8.0f;             // log2 units
+constexpr int kTmemCols = 512;             // S/P: tile x buffer x 64, O: tile x D
+constexpr int kRegionQ = kRows * 128;      // 64 columns of a query tile
+constexpr int kRegionK = kBN * 128;        // 64 columns of a block
+
+template <int D>
+struct Smem {
+  static constexpr int kQ = 0;
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kKV = 2 * kQBytes;
+  static constexpr int kKBytes = kBN * D * 2;
+  static constexpr int kBars = kKV + kStages * 2 * kKBytes;
+  static constexpr int kBytes = kBars + 256 + 1024;
+};
+static_assert(Smem<128>::kBytes <= 232448, "shared memory exceeds 227 KB");
+
+struct Params {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  const uint8_t* k;
+  const uint8_t* v;
+  const int8_t* k_exp;
+  const int8_t* v_exp;
+  int num_pages;
+  const int* block_table;
+  int64_t bt_stride;
+  int bt_pages;
+  const int* cu_q;
+  const int* kv_lens;
+  int batch, q_rows, hq, hkv, G, tpt;      // tpt: tokens per 128-row tile
+  float scale_log2;
+  int window, sinks;
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  int splits;
+  float* part_o;                           // [splits][q_rows * hq][D]
+  float2* part_ml;                         // [splits][q_rows * hq]
+  int* status;
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+      "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+      "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D (tmem) (+)= A (tmem, bf16 pairs along the columns) * B (smem descriptor)
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      " .reg .pred p;\n"
+      " setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Shared-memory descriptor of an MN-major operand, 128-byte swizzle: rows of 64 bf16 along MN, 8-row
+// atoms 1024 bytes apart along K, blocks of 64 columns `lbo` bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t smem_addr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int site) {
+  const bool ok = mbar_wait(bar, parity, abort_flag, status, kWaitTimeoutNs, kStatusWaitSite + site);
+  return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Multipliers that turn shifted e4m3 bits into values.  A code's 4 + 3 bits placed below the sign of
+// a bf16 read as code * 2^-120 (subnormal codes included), so a row's factor is 2^(120 + e): one bf16
+// while e <= 7, else two.
+struct RowScale {
+  uint32_t f, more;
+  bool two;
+};
+__device__ __forceinline__ uint32_t bf16x2_pow2(int n) { return static_cast<uint32_t>(n + 127) * 0x00800080u; }
+
+__device__ __forceinline__ RowScale row_scale(int e) {
+  RowScale s;
+  e = max(kExpMin, min(kExpMax, e));
+  s.two = e > 7;
+  s.f = bf16x2_pow2(120 + min(e, 7));
+  s.more = bf16x2_pow2(max(e - 7, 0));
+  return s;
+}
+
+// 4 codes -> 4 bf16 values
+__device__ __forceinline__ uint2 expand4(uint32_t w, const RowScale& s) {
+  uint2 o;
+  uint32_t a = __byte_perm(w, 0u, 0x1404), b = __byte_perm(w, 0u, 0x3424);
+  a = ((a >> 4) & 0x07f007f0u) | (a & 0x80008000u);
+  b = ((b >> 4) & 0x07f007f0u) | (b & 0x80008000u);
+  o.x = bf16x2_mul(a, s.f);
+  o.y = bf16x2_mul(b, s.f);
+  if (s.two) {
+    o.x = bf16x2_mul(o.x, s.more);
+    o.y = bf16x2_mul(o.y, s.more);
+  }
+  return o;
+}
+
+// This thread's share of a block: 16 codes of N rows of K and of V.
+template <int N>
+struct Share {
+  uint4 k[N], v[N];
+  int ke[N], ve[N];
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const Params p) {
+  using S = Smem<D>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* q_full = bars;                     // [2] tile
+  uint64_t* kv_full = q_full + 2;              // [kStages]
+  uint64_t* kv_empty = kv_full + kStages;      // [kStages]
+  uint64_t* s_full = kv_empty + kStages;       // [2][2] tile, buffer
+  uint64_t* p_full = s_full + 4;               // [2][2]
+  uint64_t* pv_done = p_full + 4;              // [2] tile
+  uint64_t* drain = pv_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dep_launch();
+
+  // row tile of this CTA, the last ones (with the most keys) first
+  int req = -1, tok0 = 0;
+  {
+    const int step = 2 * p.tpt;
+    int total = 0;
+    for (int base = 0; base < p.batch; base += 32) {
+      int n = 0;
+      if (base + lane < p.batch) n = (max(0, p.cu_q[base + lane + 1] - p.cu_q[base + lane]) + step - 1) / step;
+      total += __reduce_add_sync(0xffffffffu, n);
+    }
+    const int x = total - 1 - static_cast<int>(blockIdx.x);
+    if (x < 0) return;
+    int cum = 0;
+    for (int base = 0; base < p.batch && req < 0; base += 32) {
+      int n = 0;
+      if (base + lane < p.batch) n = (max(0, p.cu_q[base + lane + 1] - p.cu_q[base + lane]) + step - 1) / step;
+      int inc = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += up;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, cum + inc > x);
+      if (past != 0) {
+        const int at = __ffs(past) - 1;
+        req = base + at;
+        tok0 = (x - cum - __shfl_sync(0xffffffffu, inc - n, at)) * step;
+      }
+      cum += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  }
+  const int h = blockIdx.y, z = blockIdx.z;
+  const int q_begin = max(0, p.cu_q[req]);
+  const int q_len = min(p.cu_q[req + 1], p.q_rows) - q_begin;   // cu_q never names rows past q
+  const int kv_len = max(0, min(p.kv_lens[req], p.bt_pages * kPage));
+  const int past = kv_len - (p.cu_q[req + 1] - q_begin);        // keys before the chunk's first query
+  const int tiles = q_len - tok0 > p.tpt ? 2 : 1;
+  // keys that some row of these tiles sees: [0, sinks) and [lo, end)
+  const int end = max(0, min(kv_len, past + min(q_len, tok0 + 2 * p.tpt)));
+  const int lo = p.window > 0 ? min(end, max(0, past + tok0 - p.window + 1)) : 0;
+  const int sinks = min(p.sinks, lo);
+  const int first = lo >> 6;
+  const int sink_blocks = min((sinks + 63) >> 6, first);
+  const int blocks = end > 0 ? sink_blocks + ((end + 63) >> 6) - first : 0;
+  const int j0 = static_cast<int>(static_cast<int64_t>(blocks) * z / p.splits);
+  const int nb = static_cast<int>(static_cast<int64_t>(blocks) * (z + 1) / p.splits) - j0;
+  auto block_of = [&](int j) { return j0 + j < sink_blocks ? j0 + j : first + j0 + j - sink_blocks; };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 128);
+      mbar_init(&pv_done[i], 1);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&kv_full[i], kLoaders / 32);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto s_col = [](int t, int b) -> uint32_t { return static_cast<uint32_t>(t * 2 + b) * 64u; };
+  auto o_col = [](int t) -> uint32_t { return 256u + static_cast<uint32_t>(t) * D; };
+
+  if (warp >= 8 && warp < 12) {
+    // ------------------------------------------------------------ loaders
+    constexpr int CH = D / 16;              // 16-code chunks of a row
+    constexpr int RP = kLoaders / CH;       // rows per pass
+    constexpr int N = kBN / RP;
+    const int tid = threadIdx.x - 256;
+    const int c = tid % CH, r0 = tid / CH;
+    const int* table = p.block_table + static_cast<int64_t>(req) * p.bt_stride;
+    auto page_of = [&](int j) { return j < nb ? checked_page(table[block_of(j)], p.num_pages) : 0; };
+    auto fetch = [&](int j, int page, Share<N>& x) {
+      const int64_t row0 = (static_cast<int64_t>(page) * p.hkv + h) * kPage;
+      const int left = kv_len - block_of(j) * kPage;      // rows past the context become zeros
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = r0 + i * RP;
+        x.k[i] = x.v[i] = make_uint4(0u, 0u, 0u, 0u);
+        x.ke[i] = x.ve[i] = 0;
+        if (r < left) {
+          x.k[i] = __ldg(reinterpret_cast<const uint4*>(p.k + (row0 + r) * D + c * 16));
+          x.v[i] = __ldg(reinterpret_cast<const uint4*>(p.v + (row0 + r) * D + c * 16));
+          x.ke[i] = __ldg(p.k_exp + row0 + r);
+          x.ve[i] = __ldg(p.v_exp + row0 + r);
+        }
+      }
+    };
+    Share<N> cur;
+    int page = page_of(0);
+    if (nb > 0) fetch(0, page, cur);
+    page = page_of(1);
+    for (int j = 0; j < nb; ++j) {
+      Share<N> nxt;
+      if (j + 1 < nb) fetch(j + 1, page, nxt);
+      page = page_of(j + 2);
+      const int s = j % kStages;
+      if (j >= kStages && !warp_wait(&kv_empty[s], ((j / kStages) & 1) ^ 1, abort_flag, p.status, 41)) break;
+      uint8_t* dk = smem + S::kKV + s * 2 * S::kKBytes;
+      uint8_t* dv = dk + S::kKBytes;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = r0 + i * RP;
+        const bool bad = cur.ke[i] == kExpBad || cur.ve[i] == kExpBad;
+        RowScale ks = row_scale(cur.ke[i]), vs = row_scale(cur.ve[i]);
+        if (bad) {
+          ks.f = 0x7fc07fc0u;
+          cur.v[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        const int at = (c >> 2) * kRegionK + r * 128;
+        const int ch = 2 * (c & 3);
+        const uint2 a0 = expand4(cur.k[i].x, ks), a1 = expand4(cur.k[i].y, ks);
+        const uint2 a2 = expand4(cur.k[i].z, ks), a3 = expand4(cur.k[i].w, ks);
+        const uint2 b0 = expand4(cur.v[i].x, vs), b1 = expand4(cur.v[i].y, vs);
+        const uint2 b2 = expand4(cur.v[i].z, vs), b3 = expand4(cur.v[i].w, vs);
+        *reinterpret_cast<uint4*>(dk + at + ((ch ^ (r & 7)) << 4)) = make_uint4(a0.x, a0.y, a1.x, a1.y);
+        *reinterpret_cast<uint4*>(dk + at + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(a2.x, a2.y, a3.x, a3.y);
+        *reinterpret_cast<uint4*>(dv + at + ((ch ^ (r & 7)) << 4)) = make_uint4(b0.x, b0.y, b1.x, b1.y);
+        *reinterpret_cast<uint4*>(dv + at + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(b2.x, b2.y, b3.x, b3.y);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kv_full[s]);
+      cur = nxt;
+    }
+  } else if (warp == 12) {
+    // ------------------------------------------------------------ MMA issuer
+    constexpr uint32_t idesc_s = umma_idesc_bf16_f32(kRows, kBN);
+    constexpr uint32_t idesc_o = umma_idesc_bf16_f32(kRows, D) | (1u << 16);   // B MN-major
+    bool ok = nb > 0;
+    auto issue_s = [&](int t, int j) -> bool {
+      const int s = j % kStages;
+      if (t == 0 && !warp_wait(&kv_full[s], (j / kStages) & 1, abort_flag, p.status, 42)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t qa = smem_u32(smem + S::kQ + t * S::kQBytes);
+        const uint32_t ka = smem_u32(smem + S::kKV + s * 2 * S::kKBytes);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_f16_ss(tmem + s_col(t, j & 1), umma_desc_sw128(qa + (kk >> 2) * kRegionQ) + 2 * (kk & 3),
+                      umma_desc_sw128(ka + (kk >> 2) * kRegionK) + 2 * (kk & 3), idesc_s, kk > 0 ? 1u : 0u);
+        umma_commit(&s_full[t * 2 + (j & 1)]);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto issue_pv = [&](int t, int j) -> bool {
+      if (!warp_wait(&p_full[t * 2 + (j & 1)], (j >> 1) & 1, abort_flag, p.status, 43)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t va = smem_u32(smem + S::kKV + (j % kStages) * 2 * S::kKBytes + S::kKBytes);
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk)
+          umma_f16_ts(tmem + o_col(t), tmem + s_col(t, j & 1) + kk * 8, umma_desc_mn(va + kk * 16 * 128, kRegionK), idesc_o,
+                      (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&pv_done[t]);
+        if (t == tiles - 1) umma_commit(&kv_empty[j % kStages]);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int t = 0; t < tiles && ok; ++t) ok = warp_wait(&q_full[t], 0, abort_flag, p.status, 44);
+    for (int j = 0; j < 2 && j < nb && ok; ++j)
+      for (int t = 0; t < tiles && ok; ++t) ok = issue_s(t, j);
+    for (int j = 0; j < nb && ok; ++j) {
+      for (int t = 0; t < tiles && ok; ++t) ok = issue_pv(t, j);
+      // S of block j + 2 takes the columns that PV of block j reads P from
+      for (int t = 0; t < tiles && ok && j + 2 < nb; ++t)
+        ok = warp_wait(&pv_done[t], j & 1, abort_flag, p.status, 48) && issue_s(t, j + 2);
+    }
+    if (lane == 0) {
+      umma_commit(drain);
+      mbar_wait(drain, 0, nullptr, p.status);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax + epilogue
+    const int t = warp >> 2;
+    const int r = threadIdx.x & 127;                  // row of the tile = TMEM lane
+    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int in = r / p.G;                           // token of the row within the tile
+    const int tok = tok0 + t * p.tpt + in;
+    const int head = h * p.G + (r - in * p.G);
+    const bool row_ok = t < tiles && in < p.tpt && tok < q_len;
+    if (t < tiles && nb > 0) {
+      const __nv_bfloat16* src = p.q + static_cast<int64_t>(q_begin + (row_ok ? tok : 0)) * p.q_stride + static_cast<int64_t>(head) * D;
+      uint8_t* dst = smem + S::kQ + t * S::kQBytes + r * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 x = row_ok ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * kRegionQ + (((c & 7) ^ (r & 7)) << 4)) = x;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&q_full[t]);
+    }
+    // a row without a query keeps every key: its results are not stored
+    const int qpos = row_ok ? past + tok : 0x3fffffff;
+    const int low = row_ok && p.window > 0 ? qpos - p.window : -1;   // keys <= low are seen only below `sinks`
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    const int n = t < tiles ? nb : 0;
+    for (int j = 0; j < n && ok; ++j) {
+      const int b = j & 1;
+      if (!warp_wait(&s_full[t * 2 + b], (j >> 1) & 1, abort_flag, p.status, 45)) { ok = false; break; }
+      tc_fence_after();
+      float s[kBN];
+      {
+        uint32_t v[kBN];
+        tmem_ld32(tmem + lane_addr + s_col(t, b), v);
+        tmem_ld32(tmem + lane_addr + s_col(t, b) + 32, v + 32);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < kBN; ++i) s[i] = __uint_as_float(v[i]);
+      }
+      const int k0 = block_of(j) * kPage;
+      if (k0 + kBN - 1 > qpos || (k0 <= low && k0 + kBN > p.sinks)) {
+#pragma unroll
+        for (int i = 0; i < kBN; ++i) {
+          const int key = k0 + i;
+          s[i] = key <= qpos && (key > low || key < p.sinks) ? s[i] : -INFINITY;
+        }
+      }
+      float mx[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx[i] = s[i];
+#pragma unroll
+      for (int i = 8; i < kBN; ++i) mx[i & 7] = fmaxf(mx[i & 7], s[i]);
+      const float mraw = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+      const float mb = mraw * p.scale_log2;           // scale > 0: -inf stays -inf
+      // decided per row, executed per warp: tensor-memory accesses are warp-collective
+      const bool grow = mb > m_run + kRaise || (m_run == -INFINITY && mb > -INFINITY);
+      if (__any_sync(0xffffffffu, grow)) {
+        const bool scale_o = grow && j > 0 && m_run > -INFINITY;
+        if (__any_sync(0xffffffffu, scale_o)) {
+          if (!warp_wait(&pv_done[t], (j - 1) & 1, abort_flag, p.status, 46)) { ok = false; break; }
+          tc_fence_after();
+          const float f = scale_o ? ex2(m_run - mb) : 1.f;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t v[32];
+            tmem_ld32(tmem + lane_addr + o_col(t) + c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+            tmem_st32(tmem + lane_addr + o_col(t) + c, v);
+          }
+          tmem_st_wait();
+          l_run *= f;
+        }
+        if (grow) m_run = mb;
+      }
+      const float msub = m_run == -INFINITY ? 0.f : m_run;
+      float ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      uint32_t pk[kBN / 2];
+#pragma unroll
+      for (int i = 0; i < kBN; i += 2) {
+        const float e0 = ex2(fmaf(s[i], p.scale_log2, -msub)), e1 = ex2(fmaf(s[i + 1], p.scale_log2, -msub));
+        ls[i & 7] += e0;
+        ls[(i & 7) + 1] += e1;
+        pk[i / 2] = pack_bf16x2(e0, e1);
+      }
+      tmem_st32(tmem + lane_addr + s_col(t, b), pk);
+      l_run += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[t * 2 + b]);
+    }
+    // S of the last block came after PV of block n - 3, so two phases may still be open: in order
+    if (n > 1 && ok) ok = warp_wait(&pv_done[t], (n - 2) & 1, abort_flag, p.status, 47);
+    if (n > 0 && ok) ok = warp_wait(&pv_done[t], (n - 1) & 1, abort_flag, p.status, 47);
+    if (t < tiles && ok) {
+      tc_fence_after();
+      const int64_t row = static_cast<int64_t>(q_begin + tok) * p.hq + head;
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+      __nv_bfloat16* orow = p.out + static_cast<int64_t>(q_begin + tok) * p.out_stride + static_cast<int64_t>(head) * D;
+      float* prow = p.part_o + (static_cast<int64_t>(z) * p.q_rows * p.hq + row) * D;
+      if (p.splits > 1 && row_ok) p.part_ml[static_cast<int64_t>(z) * p.q_rows * p.hq + row] = make_float2(m_run, l_run);
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t v[32];
+        if (n > 0) {
+          tmem_ld32(tmem + lane_addr + o_col(t) + c, v);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0u;
+        }
+        if (!row_ok) continue;
+        if (p.splits > 1) {
+          if (n > 0) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(prow + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 o;
+            o.x = pack_bf16x2(__uint_as_float(v[i]) * inv, __uint_as_float(v[i + 1]) * inv);
+            o.y = pack_bf16x2(__uint_as_float(v[i + 2]) * inv, __uint_as_float(v[i + 3]) * inv);
+            o.z = pack_bf16x2(__uint_as_float(v[i + 4]) * inv, __uint_as_float(v[i + 5]) * inv);
+            o.w = pack_bf16x2(__uint_as_float(v[i + 6]) * inv, __uint_as_float(v[i + 7]) * inv);
+            *reinterpret_cast<uint4*>(orow + c + i) = o;
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Joins the splits' partial outputs of each row in order.  One warp per (token, query head); a
+// token that no request names keeps what the output held.
+template <int D>
+__global__ void __launch_bounds__(128) kv8_prefill_join_kernel(const Params p) {
+  grid_dep_wait();
+  const int64_t rows = static_cast<int64_t>(p.q_rows) * p.hq;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int64_t tok = row / p.hq;
+  if (tok >= p.cu_q[p.batch]) return;
+  constexpr int PER = D / 32;
+  float mm = -INFINITY;
+  for (int z = lane; z < p.splits; z += 32) mm = fmaxf(mm, p.part_ml[z * rows + row].x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+  float acc[PER], ll = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int z = 0; z < p.splits; ++z) {
+    const float2 v = p.part_ml[z * rows + row];
+    if (v.y == 0.f) continue;                          // a split without a visible key
+    const float f = v.x == -INFINITY ? 1.f : ex2(v.x - mm);   // without a maximum: a NaN to pass on
+    const float* src = p.part_o + (z * rows + row) * D + lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] += src[i] * f;
+    ll += v.y * f;
+  }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  __nv_bfloat16* out = p.out + tok * p.out_stride + (row - tok * p.hq) * D + lane * PER;
+#pragma unroll
+  for (int i = 0; i < PER; i += 2)
+    *reinterpret_cast<__nv_bfloat162*>(out + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
+}
+
+template <int D>
+cudaError_t launch(const Params& p, int tiles, cudaStream_t stream) {
+  cudaError_t e = ensure_smem_attr<kv8_prefill_kernel<D>>(Smem<D>::kBytes);
+  if (e != cudaSuccess) return e;
+  kv8_prefill_kernel<D><<<dim3(tiles, p.hkv, p.splits), kThreads, Smem<D>::kBytes, stream>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || p.splits == 1) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.q_rows) * p.hq + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv8_prefill_join_kernel<D>, p);
+}
+
+int64_t row_tiles(int64_t q_rows, int batch, int group) {
+  const int64_t step = 2 * (kRows / group);
+  return std::min(q_rows, q_rows / step + batch);     // each request ends in at most one partial tile
+}
+
+}  // namespace
+
+// Splits of the key blocks: as many as keep the launch within one CTA per SM, one where the row
+// tiles alone fill the GPU.
+int kv8_prefill_splits(const Kv8AttnArgs& a, int sm_count) {
+  const int64_t base = row_tiles(a.q_rows, a.batch, a.hq / a.hkv) * a.hkv;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count / std::max<int64_t>(1, base), a.bt_pages)));
+}
+
+int64_t kv8_prefill_scratch_floats(const Kv8AttnArgs& a) {
+  return a.splits > 1 ? static_cast<int64_t>(a.splits) * a.q_rows * a.hq * (a.head_dim + 2) : 0;
+}
+
+cudaError_t kv8_prefill(const Kv8AttnArgs& a, cudaStream_t stream) {
+  if (a.q_rows == 0) return cudaSuccess;
+  const int group = a.hq / a.hkv;
+  if (group > kRows) return cudaErrorInvalidValue;
+  Params p{};
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.q_stride = a.q_stride;
+  p.k = static_cast<const uint8_t*>(a.k);
+  p.v = static_cast<const uint8_t*>(a.v);
+  p.k_exp = static_cast<const int8_t*>(a.k_exp);
+  p.v_exp = static_cast<const int8_t*>(a.v_exp);
+  p.num_pages = a.num_pages;
+  p.block_table = a.block_table;
+  p.bt_stride = a.bt_stride;
+  p.bt_pages = a.bt_pages;
+  p.cu_q = a.cu_q;
+  p.kv_lens = a.kv_lens;
+  p.batch = a.batch;
+  p.q_rows = a.q_rows;
+  p.hq = a.hq;
+  p.hkv = a.hkv;
+  p.G = group;
+  p.tpt = kRows / group;
+  p.scale_log2 = a.scale * kLog2e;
+  p.window = a.window;
+  p.sinks = a.sinks;
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.out_stride = a.out_stride;
+  p.splits = a.splits;
+  p.part_o = a.scratch;
+  p.part_ml = reinterpret_cast<float2*>(a.scratch + static_cast<int64_t>(a.splits) * a.q_rows * a.hq * a.head_dim);
+  p.status = a.status;
+  const int64_t tiles = row_tiles(a.q_rows, a.batch, group);
+  if (tiles > 0x7fffffff || a.hkv > 65535) return cudaErrorInvalidValue;
+  if (a.head_dim == 128) return launch<128>(p, static_cast<int>(tiles), stream);
+  if (a.head_dim == 64) return launch<64>(p, static_cast<int>(tiles), stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace omni

@@ -242,10 +242,13 @@ struct Kv8AttnArgs {
   void* out;               // [q_rows, hq * D] bf16 rows of out_stride
   int64_t out_stride;
   int ctas;                // decode: thread blocks of the launch (kv8_decode_ctas)
-  float* scratch;          // partial sums (kv8_decode_scratch_floats), 16-byte aligned
+  int splits;              // chunk: parts of the key blocks (kv8_prefill_splits)
+  float* scratch;          // partial sums (kv8_*_scratch_floats), 16-byte aligned
   int* status;             // bounded-wait status word, may be nullptr
 };
-cudaError_t kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream);
+int kv8_prefill_splits(const Kv8AttnArgs& a, int sm_count);
+int64_t kv8_prefill_scratch_floats(const Kv8AttnArgs& a);
+cudaError_t kv8_prefill(const Kv8AttnArgs& a, cudaStream_t stream);
 int kv8_decode_ctas(int sm_count);
 int64_t kv8_decode_scratch_floats(int ctas, int group, int head_dim);
 cudaError_t kv8_decode(const Kv8AttnArgs& a, cudaStream_t stream);
