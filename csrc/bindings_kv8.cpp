@@ -233,6 +233,11 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
       scratch = torch::empty({omni::kv8_prefill_scratch_floats(a)}, f32);
       a.scratch = scratch.data_ptr<float>();
     }
+    torch::Tensor tiles;
+    if (const int64_t bytes = omni::kv8_prefill_tile_bytes(a)) {
+      tiles = torch::empty({bytes}, k.options().dtype(at::kByte));
+      a.tiles = tiles.data_ptr();
+    }
     check_launch(omni::kv8_prefill(a, at::cuda::getCurrentCUDAStream()), "kv8_prefill_attention");
   }
   return out;

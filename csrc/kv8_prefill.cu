@@ -8,7 +8,7 @@
 // One CTA: two 128-row query tiles (GQA-packed: row r = token tok0 + r / G, head h G + r % G) that
 // share every 64-key block (one page), and a range of the blocks they see:
 //
-// * Loader warps (4) read a block's codes and exponents into registers one block ahead, turn them
+// * Loader warps (4) read a block's codes and exponents into registers two blocks ahead, turn them
 //   into bf16 (exact: 4 significant bits times a power of two) and store them in the swizzled layout
 //   the tensor cores read; the cache's bytes cross HBM once per CTA at half of bf16's.
 // * One warp issues S = Q K^T and O += P V with S, P and O in tensor memory.  S has two buffers per
@@ -43,7 +43,7 @@ constexpr int kRows = 128;                 // rows of a query tile
 constexpr int kBN = kPage;                 // keys of a block
 constexpr int kStages = 5;
 constexpr int kLoaders = 128;
-constexpr int kThreads = 256 + kLoaders + 32;
+constexpr int threads(bool expanded) { return 256 + (expanded ? 32 : kLoaders) + 32; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.0f;             // log2 units
 constexpr int kTmemCols = 512;             // S/P: tile x buffer x 64, O: tile x D
@@ -82,6 +82,7 @@ struct Params {
   int splits;
   float* part_o;                           // [splits][q_rows * hq][D]
   float2* part_ml;                         // [splits][q_rows * hq]
+  uint8_t* tiles;                          // expanded K / V tiles, or nullptr
   int* status;
 };
 
@@ -122,6 +123,20 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       "}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// One lane of a converged warp.  The compiler knows the election: behind it, MMA operands stay in uniform
+// registers, where a test of the lane's number costs moves of every operand of every MMA.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
 
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -193,16 +208,111 @@ __device__ __forceinline__ uint2 expand4(uint32_t w, const RowScale& s) {
   return o;
 }
 
-// This thread's share of a block: 16 codes of N rows of K and of V.
+// This thread's share of a block: 16 codes of N consecutive rows of K and of V, and their exponents.
 template <int N>
 struct Share {
   uint4 k[N], v[N];
-  int ke[N], ve[N];
+  uint32_t ke, ve;
 };
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const Params p) {
+struct Part {
+  static constexpr int CH = D / 16;              // 16-code chunks of a row
+  static constexpr int N = kBN * CH / kLoaders;  // rows per thread
+  Share<N> x;
+  // Thread `tid` of 128 reads its share of the block whose first row is row0.
+  __device__ __forceinline__ void fetch(const Params& p, int64_t row0, int tid) {
+    row0 += tid / CH * N;
+    const uint8_t* k = p.k + row0 * D + tid % CH * 16;
+    const uint8_t* v = p.v + row0 * D + tid % CH * 16;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      x.k[i] = __ldg(reinterpret_cast<const uint4*>(k + i * D));
+      x.v[i] = __ldg(reinterpret_cast<const uint4*>(v + i * D));
+    }
+    if constexpr (N == 4) {
+      x.ke = __ldg(reinterpret_cast<const uint32_t*>(p.k_exp + row0));
+      x.ve = __ldg(reinterpret_cast<const uint32_t*>(p.v_exp + row0));
+    } else {
+      x.ke = __ldg(reinterpret_cast<const uint16_t*>(p.k_exp + row0));
+      x.ve = __ldg(reinterpret_cast<const uint16_t*>(p.v_exp + row0));
+    }
+  }
+  // Expands it into the block's K and V tiles (the tensor core's swizzled layout); rows from `left`
+  // on lie past the context: their values become zeros (their scores are masked).
+  __device__ __forceinline__ void store(uint8_t* dk, uint8_t* dv, int left, int tid) {
+    const int c = tid % CH, r0 = tid / CH * N;
+    dk += (c >> 2) * kRegionK;
+    dv += (c >> 2) * kRegionK;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = r0 + i;
+      const int ke = static_cast<int8_t>(x.ke >> (8 * i)), ve = static_cast<int8_t>(x.ve >> (8 * i));
+      const bool bad = ke == kExpBad || ve == kExpBad;
+      RowScale ks = row_scale(ke), vs = row_scale(ve);
+      if (bad) {
+        ks.f = 0x7fc07fc0u;
+        ks.two = false;
+        x.k[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      if (bad || r >= left) x.v[i] = make_uint4(0u, 0u, 0u, 0u);
+      const uint2 a0 = expand4(x.k[i].x, ks), a1 = expand4(x.k[i].y, ks);
+      const uint2 a2 = expand4(x.k[i].z, ks), a3 = expand4(x.k[i].w, ks);
+      const uint2 b0 = expand4(x.v[i].x, vs), b1 = expand4(x.v[i].y, vs);
+      const uint2 b2 = expand4(x.v[i].z, vs), b3 = expand4(x.v[i].w, vs);
+      const uint4 k0 = make_uint4(a0.x, a0.y, a1.x, a1.y), k1 = make_uint4(a2.x, a2.y, a3.x, a3.y);
+      const uint4 v0 = make_uint4(b0.x, b0.y, b1.x, b1.y), v1 = make_uint4(b2.x, b2.y, b3.x, b3.y);
+      // the two halves of a 128-dim row share banks: its lanes store their 16-byte pairs in opposite order
+      const bool swap = c >= 4;
+      const int ch = 2 * (c & 3) + (swap ? 1 : 0);
+      const int at0 = r * 128 + ((ch ^ (r & 7)) << 4), at1 = r * 128 + (((ch ^ 1) ^ (r & 7)) << 4);
+      *reinterpret_cast<uint4*>(dk + at0) = swap ? k1 : k0;
+      *reinterpret_cast<uint4*>(dk + at1) = swap ? k0 : k1;
+      *reinterpret_cast<uint4*>(dv + at0) = swap ? v1 : v0;
+      *reinterpret_cast<uint4*>(dv + at1) = swap ? v0 : v1;
+    }
+  }
+};
+
+// Key blocks that the queries at positions past .. past + n - 1 (n > 0) of a request see: the pages of
+// [0, sinks) and of [lo, end).
+struct Blocks {
+  int sink_blocks, first, count;
+  __device__ Blocks(const Params& p, int kv_len, int past, int n) {
+    const int end = max(0, min(kv_len, past + n));
+    const int lo = p.window > 0 ? min(end, max(0, past - p.window + 1)) : 0;
+    first = lo >> 6;
+    sink_blocks = min((min(p.sinks, lo) + 63) >> 6, first);
+    count = end > 0 ? sink_blocks + ((end + 63) >> 6) - first : 0;
+  }
+  __device__ int at(int j) const { return j < sink_blocks ? j : first + j - sink_blocks; }
+};
+
+// Expands every block that a request's new tokens see, once, into `tiles` (K tile, V tile of each
+// [request][page][KV head], as they will lie in shared memory).
+template <int D>
+__global__ void __launch_bounds__(kLoaders) kv8_expand_kernel(const Params p) {
+  grid_dep_launch();
+  const int req = blockIdx.y, h = blockIdx.z;
+  const int n = p.cu_q[req + 1] - p.cu_q[req];
+  const int kv_len = max(0, min(p.kv_lens[req], p.bt_pages * kPage));
+  if (n <= 0) return;
+  const Blocks bl(p, kv_len, kv_len - n, n);
+  if (static_cast<int>(blockIdx.x) >= bl.count) return;
+  const int i = bl.at(blockIdx.x);
+  const int page = checked_page(p.block_table[static_cast<int64_t>(req) * p.bt_stride + i], p.num_pages);
+  Part<D> part;
+  part.fetch(p, (static_cast<int64_t>(page) * p.hkv + h) * kPage, threadIdx.x);
+  uint8_t* dst = p.tiles + ((static_cast<int64_t>(req) * p.bt_pages + i) * p.hkv + h) * (2 * Smem<D>::kKBytes);
+  part.store(dst, dst + Smem<D>::kKBytes, kv_len - i * kPage, threadIdx.x);
+}
+
+// kExpanded: the K / V tiles come ready from kv8_expand_kernel by bulk copies, one loader warp.
+template <int D, bool kExpanded>
+__global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(const Params p) {
   using S = Smem<D>;
+  constexpr int kLoadWarps = kExpanded ? 1 : kLoaders / 32;
+  constexpr int kMmaWarp = 8 + kLoadWarps;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
@@ -215,8 +325,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const Params p
   uint64_t* drain = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   grid_dep_launch();
+  grid_dep_wait();
 
   // row tile of this CTA, the last ones (with the most keys) first
   int req = -1, tok0 = 0;
@@ -255,16 +366,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const Params p
   const int kv_len = max(0, min(p.kv_lens[req], p.bt_pages * kPage));
   const int past = kv_len - (p.cu_q[req + 1] - q_begin);        // keys before the chunk's first query
   const int tiles = q_len - tok0 > p.tpt ? 2 : 1;
-  // keys that some row of these tiles sees: [0, sinks) and [lo, end)
-  const int end = max(0, min(kv_len, past + min(q_len, tok0 + 2 * p.tpt)));
-  const int lo = p.window > 0 ? min(end, max(0, past + tok0 - p.window + 1)) : 0;
-  const int sinks = min(p.sinks, lo);
-  const int first = lo >> 6;
-  const int sink_blocks = min((sinks + 63) >> 6, first);
-  const int blocks = end > 0 ? sink_blocks + ((end + 63) >> 6) - first : 0;
-  const int j0 = static_cast<int>(static_cast<int64_t>(blocks) * z / p.splits);
-  const int nb = static_cast<int>(static_cast<int64_t>(blocks) * (z + 1) / p.splits) - j0;
-  auto block_of = [&](int j) { return j0 + j < sink_blocks ? j0 + j : first + j0 + j - sink_blocks; };
+  const Blocks bl(p, kv_len, past + tok0, min(q_len - tok0, 2 * p.tpt));
+  const int j0 = static_cast<int>(static_cast<int64_t>(bl.count) * z / p.splits);
+  const int nb = static_cast<int>(static_cast<int64_t>(bl.count) * (z + 1) / p.splits) - j0;
+  auto block_of = [&](int j) { return bl.at(j0 + j); };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -272,18 +377,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const Params p
       mbar_init(&pv_done[i], 1);
     }
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&kv_full[i], kLoaders / 32);
+      mbar_init(&kv_full[i], kLoadWarps);
       mbar_init(&kv_empty[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], 4);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
@@ -294,114 +399,115 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const Params p
   auto s_col = [](int t, int b) -> uint32_t { return static_cast<uint32_t>(t * 2 + b) * 64u; };
   auto o_col = [](int t) -> uint32_t { return 256u + static_cast<uint32_t>(t) * D; };
 
-  if (warp >= 8 && warp < 12) {
+  if (warp >= 8 && warp < kMmaWarp) {
     // ------------------------------------------------------------ loaders
-    constexpr int CH = D / 16;              // 16-code chunks of a row
-    constexpr int RP = kLoaders / CH;       // rows per pass
-    constexpr int N = kBN / RP;
-    const int tid = threadIdx.x - 256;
-    const int c = tid % CH, r0 = tid / CH;
-    const int* table = p.block_table + static_cast<int64_t>(req) * p.bt_stride;
-    auto page_of = [&](int j) { return j < nb ? checked_page(table[block_of(j)], p.num_pages) : 0; };
-    auto fetch = [&](int j, int page, Share<N>& x) {
-      const int64_t row0 = (static_cast<int64_t>(page) * p.hkv + h) * kPage;
-      const int left = kv_len - block_of(j) * kPage;      // rows past the context become zeros
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int r = r0 + i * RP;
-        x.k[i] = x.v[i] = make_uint4(0u, 0u, 0u, 0u);
-        x.ke[i] = x.ve[i] = 0;
-        if (r < left) {
-          x.k[i] = __ldg(reinterpret_cast<const uint4*>(p.k + (row0 + r) * D + c * 16));
-          x.v[i] = __ldg(reinterpret_cast<const uint4*>(p.v + (row0 + r) * D + c * 16));
-          x.ke[i] = __ldg(p.k_exp + row0 + r);
-          x.ve[i] = __ldg(p.v_exp + row0 + r);
+    int stage = 0;
+    uint32_t phase = 1;                     // the first round finds the ring empty
+    if constexpr (kExpanded) {
+      if (elect_one()) {
+        const uint8_t* src = p.tiles + (static_cast<int64_t>(req) * p.bt_pages * p.hkv + h) * (2 * S::kKBytes);
+        int j = 0;
+        for (; j < nb; ++j) {
+          if (j >= kStages && !mbar_wait(&kv_empty[stage], phase, abort_flag, p.status, kWaitTimeoutNs, kStatusWaitSite + 41)) break;
+          mbar_arrive_expect_tx(&kv_full[stage], 2 * S::kKBytes);
+          bulk_copy(smem + S::kKV + stage * 2 * S::kKBytes, src + static_cast<int64_t>(block_of(j)) * p.hkv * (2 * S::kKBytes),
+                    2 * S::kKBytes, &kv_full[stage]);
+          if (++stage == kStages) stage = 0, phase ^= 1;
         }
+        // every issued copy has landed before the CTA's shared memory goes away
+        for (int i = max(0, j - kStages); i < j; ++i) mbar_wait(&kv_full[i % kStages], (i / kStages) & 1, nullptr, p.status);
       }
-    };
-    Share<N> cur;
-    int page = page_of(0);
-    if (nb > 0) fetch(0, page, cur);
-    page = page_of(1);
-    for (int j = 0; j < nb; ++j) {
-      Share<N> nxt;
-      if (j + 1 < nb) fetch(j + 1, page, nxt);
-      page = page_of(j + 2);
-      const int s = j % kStages;
-      if (j >= kStages && !warp_wait(&kv_empty[s], ((j / kStages) & 1) ^ 1, abort_flag, p.status, 41)) break;
-      uint8_t* dk = smem + S::kKV + s * 2 * S::kKBytes;
-      uint8_t* dv = dk + S::kKBytes;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int r = r0 + i * RP;
-        const bool bad = cur.ke[i] == kExpBad || cur.ve[i] == kExpBad;
-        RowScale ks = row_scale(cur.ke[i]), vs = row_scale(cur.ve[i]);
-        if (bad) {
-          ks.f = 0x7fc07fc0u;
-          cur.v[i] = make_uint4(0u, 0u, 0u, 0u);
-        }
-        const int at = (c >> 2) * kRegionK + r * 128;
-        const int ch = 2 * (c & 3);
-        const uint2 a0 = expand4(cur.k[i].x, ks), a1 = expand4(cur.k[i].y, ks);
-        const uint2 a2 = expand4(cur.k[i].z, ks), a3 = expand4(cur.k[i].w, ks);
-        const uint2 b0 = expand4(cur.v[i].x, vs), b1 = expand4(cur.v[i].y, vs);
-        const uint2 b2 = expand4(cur.v[i].z, vs), b3 = expand4(cur.v[i].w, vs);
-        *reinterpret_cast<uint4*>(dk + at + ((ch ^ (r & 7)) << 4)) = make_uint4(a0.x, a0.y, a1.x, a1.y);
-        *reinterpret_cast<uint4*>(dk + at + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(a2.x, a2.y, a3.x, a3.y);
-        *reinterpret_cast<uint4*>(dv + at + ((ch ^ (r & 7)) << 4)) = make_uint4(b0.x, b0.y, b1.x, b1.y);
-        *reinterpret_cast<uint4*>(dv + at + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(b2.x, b2.y, b3.x, b3.y);
-      }
-      fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&kv_full[s]);
-      cur = nxt;
+    } else {
+      const int tid = threadIdx.x - 256;
+      const int* table = p.block_table + static_cast<int64_t>(req) * p.bt_stride;
+      auto page_of = [&](int j) { return j < nb ? checked_page(table[block_of(j)], p.num_pages) : 0; };
+      auto fetch = [&](int j, int page, Part<D>& x) {
+        if (j < nb) x.fetch(p, (static_cast<int64_t>(page) * p.hkv + h) * kPage, tid);
+      };
+      Part<D> buf[3];                       // blocks j, j + 1, j + 2
+      bool ok = true;
+      int page = page_of(2);
+      fetch(0, page_of(0), buf[0]);
+      fetch(1, page_of(1), buf[1]);
+      auto put = [&](int j, Part<D>& cur, Part<D>& far) {
+        fetch(j + 2, page, far);
+        page = page_of(j + 3);
+        if (j >= kStages) ok = warp_wait(&kv_empty[stage], phase, abort_flag, p.status, 41);
+        if (!ok) return;
+        uint8_t* dk = smem + S::kKV + stage * 2 * S::kKBytes;
+        cur.store(dk, dk + S::kKBytes, kv_len - block_of(j) * kPage, tid);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[stage]);
+        if (++stage == kStages) stage = 0, phase ^= 1;
+      };
+      for (int j = 0; j < nb && ok; j += 3) {
+        put(j, buf[0], buf[2]);
+        if (j + 1 < nb && ok) put(j + 1, buf[1], buf[0]);
+        if (j + 2 < nb && ok) put(j + 2, buf[2], buf[1]);
+      }
     }
-  } else if (warp == 12) {
+  } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
-    constexpr uint32_t idesc_s = umma_idesc_bf16_f32(kRows, kBN);
-    constexpr uint32_t idesc_o = umma_idesc_bf16_f32(kRows, D) | (1u << 16);   // B MN-major
-    bool ok = nb > 0;
-    auto issue_s = [&](int t, int j) -> bool {
-      const int s = j % kStages;
-      if (t == 0 && !warp_wait(&kv_full[s], (j / kStages) & 1, abort_flag, p.status, 42)) return false;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t qa = smem_u32(smem + S::kQ + t * S::kQBytes);
-        const uint32_t ka = smem_u32(smem + S::kKV + s * 2 * S::kKBytes);
+    // One thread runs the whole sequence: its instructions between two MMAs are what the tensor
+    // core waits for, so the descriptors are a base plus constants and nothing is warp-wide.
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = umma_idesc_bf16_f32(kRows, kBN);
+      constexpr uint32_t idesc_o = umma_idesc_bf16_f32(kRows, D) | (1u << 16);   // B MN-major
+      const uint64_t dq = umma_desc_sw128(smem_u32(smem + S::kQ));
+      const uint64_t dk = umma_desc_sw128(smem_u32(smem + S::kKV));
+      const uint64_t dv = umma_desc_mn(smem_u32(smem + S::kKV + S::kKBytes), kRegionK);
+      auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+        return mbar_wait(bar, parity, abort_flag, p.status, kWaitTimeoutNs, kStatusWaitSite + site);
+      };
+      auto issue_s = [&](int t, int b, int s) {
+        const uint64_t qa = dq + t * (S::kQBytes >> 4), ka = dk + s * (2 * S::kKBytes >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16_ss(tmem + s_col(t, j & 1), umma_desc_sw128(qa + (kk >> 2) * kRegionQ) + 2 * (kk & 3),
-                      umma_desc_sw128(ka + (kk >> 2) * kRegionK) + 2 * (kk & 3), idesc_s, kk > 0 ? 1u : 0u);
-        umma_commit(&s_full[t * 2 + (j & 1)]);
+          umma_f16_ss(tmem + s_col(t, b), qa + ((kk >> 2) * (kRegionQ >> 4) + 2 * (kk & 3)),
+                      ka + ((kk >> 2) * (kRegionK >> 4) + 2 * (kk & 3)), idesc_s, kk > 0 ? 1u : 0u);
+        umma_commit(&s_full[t * 2 + b]);
+      };
+      bool ok = nb > 0;
+      for (int t = 0; t < tiles && ok; ++t) ok = wait(&q_full[t], 0, 44);
+      int ss = 0;                 // ring stage and phase of the next S
+      uint32_t sp = 0;
+      for (int j = 0; j < 2 && j < nb && ok; ++j) {
+        ok = wait(&kv_full[ss], sp, 42);
+        if (!ok) break;
+        tc_fence_after();
+        for (int t = 0; t < tiles; ++t) issue_s(t, j, ss);
+        if (++ss == kStages) ss = 0, sp ^= 1;
       }
-      __syncwarp();
-      return true;
-    };
-    auto issue_pv = [&](int t, int j) -> bool {
-      if (!warp_wait(&p_full[t * 2 + (j & 1)], (j >> 1) & 1, abort_flag, p.status, 43)) return false;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t va = smem_u32(smem + S::kKV + (j % kStages) * 2 * S::kKBytes + S::kKBytes);
+      int ps = 0;                 // ring stage of the next PV
+      for (int j = 0; j < nb && ok; ++j) {
+        const int b = j & 1;
+        for (int t = 0; t < tiles; ++t) {
+          ok = wait(&p_full[t * 2 + b], (j >> 1) & 1, 43);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t va = dv + ps * (2 * S::kKBytes >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kBN / 16; ++kk)
-          umma_f16_ts(tmem + o_col(t), tmem + s_col(t, j & 1) + kk * 8, umma_desc_mn(va + kk * 16 * 128, kRegionK), idesc_o,
-                      (j > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&pv_done[t]);
-        if (t == tiles - 1) umma_commit(&kv_empty[j % kStages]);
+          for (int kk = 0; kk < kBN / 16; ++kk)
+            umma_f16_ts(tmem + o_col(t), tmem + s_col(t, b) + kk * 8, va + kk * (16 * 128 >> 4), idesc_o,
+                        (j > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&pv_done[t]);
+          if (t == tiles - 1) umma_commit(&kv_empty[ps]);
+        }
+        if (!ok) break;
+        if (++ps == kStages) ps = 0;
+        if (j + 2 < nb) {
+          ok = wait(&kv_full[ss], sp, 42);
+          // S of block j + 2 takes the columns that PV of block j reads P from
+          for (int t = 0; t < tiles && ok; ++t) {
+            ok = wait(&pv_done[t], b, 48);
+            tc_fence_after();
+            if (ok) issue_s(t, b, ss);
+          }
+          if (++ss == kStages) ss = 0, sp ^= 1;
+        }
       }
-      __syncwarp();
-      return true;
-    };
-    for (int t = 0; t < tiles && ok; ++t) ok = warp_wait(&q_full[t], 0, abort_flag, p.status, 44);
-    for (int j = 0; j < 2 && j < nb && ok; ++j)
-      for (int t = 0; t < tiles && ok; ++t) ok = issue_s(t, j);
-    for (int j = 0; j < nb && ok; ++j) {
-      for (int t = 0; t < tiles && ok; ++t) ok = issue_pv(t, j);
-      // S of block j + 2 takes the columns that PV of block j reads P from
-      for (int t = 0; t < tiles && ok && j + 2 < nb; ++t)
-        ok = warp_wait(&pv_done[t], j & 1, abort_flag, p.status, 48) && issue_s(t, j + 2);
-    }
-    if (lane == 0) {
       umma_commit(drain);
       mbar_wait(drain, 0, nullptr, p.status);
     }
@@ -496,7 +602,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const Params p
       l_run += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[t * 2 + b]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t * 2 + b]);
     }
     // S of the last block came after PV of block n - 3, so two phases may still be open: in order
     if (n > 1 && ok) ok = warp_wait(&pv_done[t], (n - 2) & 1, abort_flag, p.status, 47);
@@ -541,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const Params p
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
@@ -583,23 +690,39 @@ __global__ void __launch_bounds__(128) kv8_prefill_join_kernel(const Params p) {
     *reinterpret_cast<__nv_bfloat162*>(out + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
 }
 
-template <int D>
-cudaError_t launch(const Params& p, int tiles, cudaStream_t stream) {
-  cudaError_t e = ensure_smem_attr<kv8_prefill_kernel<D>>(Smem<D>::kBytes);
-  if (e != cudaSuccess) return e;
-  kv8_prefill_kernel<D><<<dim3(tiles, p.hkv, p.splits), kThreads, Smem<D>::kBytes, stream>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || p.splits == 1) return e;
+// A launch that may start while the one before it on the stream still runs; its kernel waits.
+template <class... Args>
+cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int block, int smem, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.q_rows) * p.hq + 3) / 4));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv8_prefill_join_kernel<D>, p);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <int D>
+cudaError_t launch(const Params& p, int tiles, cudaStream_t stream) {
+  const dim3 grid(tiles, p.hkv, p.splits);
+  cudaError_t e;
+  if (p.tiles != nullptr) {
+    if ((e = ensure_smem_attr<kv8_prefill_kernel<D, true>>(Smem<D>::kBytes)) != cudaSuccess) return e;
+    kv8_expand_kernel<D><<<dim3(p.bt_pages, p.batch, p.hkv), kLoaders, 0, stream>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    e = launch_dependent(kv8_prefill_kernel<D, true>, grid, threads(true), Smem<D>::kBytes, stream, p);
+  } else {
+    if ((e = ensure_smem_attr<kv8_prefill_kernel<D, false>>(Smem<D>::kBytes)) != cudaSuccess) return e;
+    kv8_prefill_kernel<D, false><<<grid, threads(false), Smem<D>::kBytes, stream>>>(p);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess || p.splits == 1) return e;
+  const int64_t rows = static_cast<int64_t>(p.q_rows) * p.hq;
+  return launch_dependent(kv8_prefill_join_kernel<D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, p);
 }
 
 int64_t row_tiles(int64_t q_rows, int batch, int group) {
@@ -614,6 +737,14 @@ int64_t row_tiles(int64_t q_rows, int batch, int group) {
 int kv8_prefill_splits(const Kv8AttnArgs& a, int sm_count) {
   const int64_t base = row_tiles(a.q_rows, a.batch, a.hq / a.hkv) * a.hkv;
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count / std::max<int64_t>(1, base), a.bt_pages)));
+}
+
+// Bytes of the expanded tiles, 0 where the blocks are expanded in the attention kernel itself.
+int64_t kv8_prefill_tile_bytes(const Kv8AttnArgs& a) {
+  const int64_t step = 2 * (kRows / (a.hq / a.hkv));
+  const int64_t bytes = static_cast<int64_t>(a.batch) * a.bt_pages * a.hkv * kPage * a.head_dim * 4;
+  if (a.q_rows < 2 * step * a.batch || a.splits > 1 || bytes > (int64_t{1} << 31) || a.batch > 65535) return 0;
+  return bytes;
 }
 
 int64_t kv8_prefill_scratch_floats(const Kv8AttnArgs& a) {
@@ -651,6 +782,7 @@ cudaError_t kv8_prefill(const Kv8AttnArgs& a, cudaStream_t stream) {
   p.splits = a.splits;
   p.part_o = a.scratch;
   p.part_ml = reinterpret_cast<float2*>(a.scratch + static_cast<int64_t>(a.splits) * a.q_rows * a.hq * a.head_dim);
+  p.tiles = static_cast<uint8_t*>(a.tiles);
   p.status = a.status;
   const int64_t tiles = row_tiles(a.q_rows, a.batch, group);
   if (tiles > 0x7fffffff || a.hkv > 65535) return cudaErrorInvalidValue;
