@@ -322,7 +322,8 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
   uint64_t* s_full = kv_empty + kStages;       // [2][2] tile, buffer
   uint64_t* p_full = s_full + 4;               // [2][2]
   uint64_t* pv_done = p_full + 4;              // [2] tile
-  uint64_t* drain = pv_done + 2;
+  uint64_t* o_full = pv_done + 2;              // [2] tile: the last PV
+  uint64_t* drain = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -375,6 +376,7 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 128);
       mbar_init(&pv_done[i], 1);
+      mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&kv_full[i], kLoadWarps);
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
           for (int kk = 0; kk < kBN / 16; ++kk)
             umma_f16_ts(tmem + o_col(t), tmem + s_col(t, b) + kk * 8, va + kk * (16 * 128 >> 4), idesc_o,
                         (j > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&pv_done[t]);
+          umma_commit(j + 1 < nb ? &pv_done[t] : &o_full[t]);
           if (t == tiles - 1) umma_commit(&kv_empty[ps]);
         }
         if (!ok) break;
@@ -605,9 +607,8 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[t * 2 + b]);
     }
-    // S of the last block came after PV of block n - 3, so two phases may still be open: in order
-    if (n > 1 && ok) ok = warp_wait(&pv_done[t], (n - 2) & 1, abort_flag, p.status, 47);
-    if (n > 0 && ok) ok = warp_wait(&pv_done[t], (n - 1) & 1, abort_flag, p.status, 47);
+    // a barrier of its own: pv_done's phase may be one or two behind here, which its parity cannot tell
+    if (n > 0 && ok) ok = warp_wait(&o_full[t], 0, abort_flag, p.status, 47);
     if (t < tiles && ok) {
       tc_fence_after();
       const int64_t row = static_cast<int64_t>(q_begin + tok) * p.hq + head;
