@@ -473,41 +473,51 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
       };
       bool ok = nb > 0;
       for (int t = 0; t < tiles && ok; ++t) ok = wait(&q_full[t], 0, 44);
-      int ss = 0;                 // ring stage and phase of the next S
+      auto issue_pv = [&](int t, int j, int s) {
+        const uint64_t va = dv + s * (2 * S::kKBytes >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk)
+          umma_f16_ts(tmem + o_col(t), tmem + s_col(t, j & 1) + kk * 8, va + kk * (16 * 128 >> 4), idesc_o,
+                      (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(j + 1 < nb ? &pv_done[t] : &o_full[t]);
+        if (t == tiles - 1) umma_commit(&kv_empty[s]);
+      };
+      auto next = [](int s) { return s + 1 == kStages ? 0 : s + 1; };
+      // Order: PV_A(j)  S_B(j + 1)  PV_B(j)  S_A(j + 2).  S of a block takes the columns that PV two
+      // blocks before reads P from, so it waits for that PV; the other tile's two products lie in
+      // between, and keep the tensor core busy meanwhile.
+      int s0 = 0, s2 = 0;         // ring stages of blocks j and j + 2 (the next S_A)
       uint32_t sp = 0;
       for (int j = 0; j < 2 && j < nb && ok; ++j) {
-        ok = wait(&kv_full[ss], sp, 42);
+        ok = wait(&kv_full[s2], sp, 42);
         if (!ok) break;
         tc_fence_after();
-        for (int t = 0; t < tiles; ++t) issue_s(t, j, ss);
-        if (++ss == kStages) ss = 0, sp ^= 1;
+        issue_s(0, j, s2);
+        if (j == 0 && tiles == 2) issue_s(1, 0, s2);
+        s2 = next(s2);
       }
-      int ps = 0;                 // ring stage of the next PV
       for (int j = 0; j < nb && ok; ++j) {
-        const int b = j & 1;
-        for (int t = 0; t < tiles; ++t) {
-          ok = wait(&p_full[t * 2 + b], (j >> 1) & 1, 43);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t va = dv + ps * (2 * S::kKBytes >> 4);
-#pragma unroll
-          for (int kk = 0; kk < kBN / 16; ++kk)
-            umma_f16_ts(tmem + o_col(t), tmem + s_col(t, b) + kk * 8, va + kk * (16 * 128 >> 4), idesc_o,
-                        (j > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(j + 1 < nb ? &pv_done[t] : &o_full[t]);
-          if (t == tiles - 1) umma_commit(&kv_empty[ps]);
-        }
-        if (!ok) break;
-        if (++ps == kStages) ps = 0;
-        if (j + 2 < nb) {
-          ok = wait(&kv_full[ss], sp, 42);
-          // S of block j + 2 takes the columns that PV of block j reads P from
-          for (int t = 0; t < tiles && ok; ++t) {
-            ok = wait(&pv_done[t], b, 48);
+        const int b = j & 1, s1 = next(s0);
+        if (!(ok = wait(&p_full[b], (j >> 1) & 1, 43))) break;
+        tc_fence_after();
+        issue_pv(0, j, s0);
+        if (tiles == 2) {
+          if (j + 1 < nb) {
+            if (j > 0 && !(ok = wait(&pv_done[1], b ^ 1, 48))) break;
             tc_fence_after();
-            if (ok) issue_s(t, b, ss);
+            issue_s(1, b ^ 1, s1);
           }
-          if (++ss == kStages) ss = 0, sp ^= 1;
+          if (!(ok = wait(&p_full[2 + b], (j >> 1) & 1, 43))) break;
+          tc_fence_after();
+          issue_pv(1, j, s0);
+        }
+        s0 = s1;
+        if (j + 2 < nb) {
+          if (!(ok = wait(&kv_full[s2], sp, 42) && wait(&pv_done[0], b, 48))) break;
+          tc_fence_after();
+          issue_s(0, b, s2);
+          s2 = next(s2);
+          if (s2 == 0) sp ^= 1;
         }
       }
       umma_commit(drain);
