@@ -159,6 +159,33 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 lanes per instruction, and a maximum of three: the softmax's arithmetic is bound by issue slots.
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -571,12 +598,12 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
           s[i] = key <= qpos && (key > low || key < p.sinks) ? s[i] : -INFINITY;
         }
       }
-      float mx[8];
+      float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mx[i] = s[i];
+      for (int i = 4; i < kBN; i += 8)
 #pragma unroll
-      for (int i = 8; i < kBN; ++i) mx[i & 7] = fmaxf(mx[i & 7], s[i]);
-      const float mraw = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+        for (int u = 0; u < 4; ++u) mx[u] = i + 4 < kBN ? max3(mx[u], s[i + u], s[i + 4 + u]) : fmaxf(mx[u], s[i + u]);
+      const float mraw = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
       const float mb = mraw * p.scale_log2;           // scale > 0: -inf stays -inf
       // decided per row, executed per warp: tensor-memory accesses are warp-collective
       const bool grow = mb > m_run + kRaise || (m_run == -INFINITY && mb > -INFINITY);
@@ -601,17 +628,19 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
         if (grow) m_run = mb;
       }
       const float msub = m_run == -INFINITY ? 0.f : m_run;
-      float ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), sub2 = f32x2(-msub, -msub);
+      uint64_t ls[4] = {0, 0, 0, 0};
       uint32_t pk[kBN / 2];
 #pragma unroll
       for (int i = 0; i < kBN; i += 2) {
-        const float e0 = ex2(fmaf(s[i], p.scale_log2, -msub)), e1 = ex2(fmaf(s[i + 1], p.scale_log2, -msub));
-        ls[i & 7] += e0;
-        ls[(i & 7) + 1] += e1;
+        const float2 x = unpack(fma2(f32x2(s[i], s[i + 1]), scale2, sub2));
+        const float e0 = ex2(x.x), e1 = ex2(x.y);
+        ls[(i >> 1) & 3] = add2(ls[(i >> 1) & 3], f32x2(e0, e1));
         pk[i / 2] = pack_bf16x2(e0, e1);
       }
       tmem_st32(tmem + lane_addr + s_col(t, b), pk);
-      l_run += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+      const float2 lsum = unpack(add2(add2(ls[0], ls[1]), add2(ls[2], ls[3])));
+      l_run += lsum.x + lsum.y;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
