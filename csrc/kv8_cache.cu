@@ -52,80 +52,70 @@ __device__ __forceinline__ int rope_axis(int j, const Kv8StoreArgs& a) {
 
 // A head row is D / 8 lanes of 8 elements (16-byte loads), so a warp takes 32 / (D / 8) heads of one
 // token at a time, `passes` such groups one after another (the next group's row is read ahead).  The
-// grid's first dimension is the token: its positions, cos and sin are read once per warp.
-// kPairs: adjacent-pair rotation; kPlain: the 8 angles of a lane lie side by side in the table (one
-// position, halves a multiple of 8), so they are read as vectors.
-template <int D, bool kPairs, bool kPlain>
-__global__ void __launch_bounds__(128) kv8_store_kernel(const Kv8StoreArgs a, int passes) {
+// grid's first dimension is the token: its angles are looked up once per block, one pair per thread.
+enum Rope : int {
+  kNone,        // no rotation
+  kPairs,       // adjacent pairs
+  kHalves,      // halves, rot / 2 a multiple of 8: the other element lies in another lane at the same place
+  kOddHalves,   // halves of any size: through shared memory
+};
+template <int D, int kRope>
+__global__ void __launch_bounds__(128, 8) kv8_store_kernel(const Kv8StoreArgs a, int passes) {
   grid_dep_launch();
   constexpr int L = D / 8;          // lanes per head
   constexpr int HW = 32 / L;        // heads per warp and pass
-  __shared__ float rows[kPairs || kPlain ? 1 : 4][HW][D];   // partner exchange of odd halves
+  __shared__ float rows[kRope == kOddHalves ? 4 : 1][HW][D];   // partner exchange
+  __shared__ __align__(16) float angle[2][D / 2];  // cos, sin of the token's pairs
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane / L, l = lane - sub * L;
   const int heads = a.hq + 2 * a.hkv;
   const int tok = blockIdx.x;
   const int head0 = (blockIdx.y * 4 + warp) * HW * passes + sub;
   const int half = a.rot_dim >> 1;
-  if (head0 - sub >= heads) return;
   const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.qkv) + static_cast<int64_t>(tok) * a.qkv_stride + l * 8;
   uint4 raw = head0 < heads ? *reinterpret_cast<const uint4*>(src + head0 * D) : make_uint4(0u, 0u, 0u, 0u);
-
-  // cos / sin of the 8 elements of this lane; s carries the sign: x1 cos - x2 sin, x2 cos + x1 sin
-  float c[8], s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    c[i] = 1.f;
-    s[i] = 0.f;
+  if (kRope != kNone && static_cast<int>(threadIdx.x) < half) {
+    const int j = threadIdx.x;
+    const int p = max(0, min(a.positions[static_cast<int64_t>(rope_axis(j, a)) * a.tokens + tok], a.max_pos - 1));
+    angle[0][j] = a.cos_tab[static_cast<int64_t>(p) * half + j];
+    angle[1][j] = a.sin_tab[static_cast<int64_t>(p) * half + j];
   }
-  if (l * 8 < a.rot_dim) {
-    if constexpr (kPlain) {
-      const int64_t p = max(0, min(a.positions[tok], a.max_pos - 1));
-      constexpr int n = kPairs ? 4 : 8;
-      const int j = kPairs ? l * 4 : (l * 8 < half ? l * 8 : l * 8 - half);
-      const float* ct = a.cos_tab + p * half + j;
-      const float* st = a.sin_tab + p * half + j;
+  __syncthreads();
+  if (head0 - sub >= heads) return;
+
+  // of this lane's 8 elements; s carries the sign: x1 cos - x2 sin, x2 cos + x1 sin
+  float c[8], s[8];
+  if (kRope == kHalves) {
+    const int j = l * 8 < half ? l * 8 : min(l * 8, a.rot_dim - 8) - half;
 #pragma unroll
-      for (int i = 0; i < n; i += 4) {
-        const float4 cv = *reinterpret_cast<const float4*>(ct + i), sv = *reinterpret_cast<const float4*>(st + i);
-        const float cc[4] = {cv.x, cv.y, cv.z, cv.w}, sc[4] = {sv.x, sv.y, sv.z, sv.w};
+    for (int i = 0; i < 8; i += 4) {
+      const float4 cv = *reinterpret_cast<const float4*>(&angle[0][j + i]), sv = *reinterpret_cast<const float4*>(&angle[1][j + i]);
+      c[i] = cv.x, c[i + 1] = cv.y, c[i + 2] = cv.z, c[i + 3] = cv.w;
+      s[i] = sv.x, s[i + 1] = sv.y, s[i + 2] = sv.z, s[i + 3] = sv.w;
+    }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if constexpr (kPairs) {
-            c[2 * u] = c[2 * u + 1] = cc[u];
-            s[2 * u] = -sc[u];
-            s[2 * u + 1] = sc[u];
-          } else {
-            c[i + u] = cc[u];
-            s[i + u] = l * 8 < half ? -sc[u] : sc[u];
-          }
-        }
-      }
-    } else {
-      int64_t at[3];
+    for (int i = 0; i < 8; ++i) s[i] = l * 8 < half ? -s[i] : s[i];
+  } else if (kRope != kNone) {
 #pragma unroll
-      for (int u = 0; u < 3; ++u) {
-        const int p = u < a.pos_rows ? a.positions[static_cast<int64_t>(u) * a.tokens + tok] : 0;
-        at[u] = static_cast<int64_t>(max(0, min(p, a.max_pos - 1))) * half;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int e = l * 8 + i;
-        if (e >= a.rot_dim) continue;
-        const int j = kPairs ? e >> 1 : (e < half ? e : e - half);
-        const int ax = rope_axis(j, a);
-        const int64_t row = ax == 0 ? at[0] : (ax == 1 ? at[1] : at[2]);
-        c[i] = a.cos_tab[row + j];
-        s[i] = a.sin_tab[row + j];
-        if (kPairs ? (i & 1) == 0 : e < half) s[i] = -s[i];
+    for (int i = 0; i < 8; ++i) {
+      const int e = l * 8 + i;
+      c[i] = 1.f;
+      s[i] = 0.f;
+      if (e < a.rot_dim) {
+        const int j = kRope == kPairs ? e >> 1 : (e < half ? e : e - half);
+        c[i] = angle[0][j];
+        s[i] = (kRope == kPairs ? (i & 1) == 0 : e < half) ? -angle[1][j] : angle[1][j];
       }
     }
   }
   const int64_t slot = a.slot_mapping[tok];
   const bool store = slot >= 0 && slot < a.num_slots;
-  float wq[8], wk[8];
-  if (a.q_norm != nullptr) unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q_norm) + l * 8), wq);
-  if (a.k_norm != nullptr) unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.k_norm) + l * 8), wk);
+  float w[8];                       // norm weights of the current kind of head
+  int kind = -1;                    // 0 q, 1 k, 2 v
+  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.q_out) + static_cast<int64_t>(tok) * a.q_out_stride + l * 8;
+  const int step = half >> 3;       // lanes between the two elements of a pair
+  const int from = sub * L + (l < step ? l + step : (l < 2 * step ? l - step : l));
+  const bool rotates = l * 8 < a.rot_dim;
 
   for (int it = 0; it < passes; ++it) {
     const int head = head0 + it * HW;
@@ -135,27 +125,29 @@ __global__ void __launch_bounds__(128) kv8_store_kernel(const Kv8StoreArgs a, in
     float x[8];
     unpack8(raw, x);
     if (it + 1 < passes && head + HW < heads) raw = *reinterpret_cast<const uint4*>(src + (head + HW) * D);
-    const bool norm = is_q ? a.q_norm != nullptr : (is_k && a.k_norm != nullptr);
-    if (__any_sync(0xffffffffu, norm)) {
+    const void* wp = is_q ? a.q_norm : (is_k ? a.k_norm : nullptr);
+    if (kind != (is_q ? 0 : (is_k ? 1 : 2))) {
+      kind = is_q ? 0 : (is_k ? 1 : 2);
+      if (wp != nullptr) unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(wp) + l * 8), w);
+    }
+    if (__any_sync(0xffffffffu, wp != nullptr)) {
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
 #pragma unroll
       for (int d = 1; d < L; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-      if (norm) {
-        const float r = rsqrtf(ss / D + a.eps);
+      if (wp != nullptr) {
+        const float r = rsqrtf(ss * (1.f / D) + a.eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (is_q ? wq[i] : wk[i]);
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
       }
     }
-    if (a.rot_dim > 0 && __any_sync(0xffffffffu, is_q || is_k)) {
+    if (kRope != kNone && __any_sync(0xffffffffu, is_q || is_k)) {
       float y[8];   // the other element of each pair
-      if constexpr (kPairs) {
+      if constexpr (kRope == kPairs) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-      } else if (kPlain || (half & 7) == 0) {
-        const int step = half >> 3;
-        const int from = sub * L + (l < step ? l + step : (l < 2 * step ? l - step : l));
+      } else if constexpr (kRope == kHalves) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], from);
       } else {
@@ -170,14 +162,17 @@ __global__ void __launch_bounds__(128) kv8_store_kernel(const Kv8StoreArgs a, in
           y[i] = row[e < half ? e + half : (e < a.rot_dim ? e - half : e)];
         }
       }
-      if (is_q || is_k) {
+      if (rotates && (is_q || is_k)) {
+        if (kRope == kHalves || (a.rot_dim & 7) == 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = l * 8 + i < a.rot_dim ? x[i] * c[i] + y[i] * s[i] : x[i];
+          for (int i = 0; i < 8; ++i) x[i] = x[i] * c[i] + y[i] * s[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = l * 8 + i < a.rot_dim ? x[i] * c[i] + y[i] * s[i] : x[i];
+        }
       }
     }
-    if (is_q)
-      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.q_out) + static_cast<int64_t>(tok) * a.q_out_stride +
-                                head * D + l * 8) = pack8(x);
+    if (is_q) *reinterpret_cast<uint4*>(dst + head * D) = pack8(x);
     if (__all_sync(0xffffffffu, is_q)) continue;
     uint32_t top = 0;
 #pragma unroll
@@ -244,28 +239,24 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8ReadArgs a) {
 
 namespace {
 
-template <int D, bool kPairs, bool kPlain>
+template <int D>
 cudaError_t launch_store(const Kv8StoreArgs& a, cudaStream_t stream) {
   const int heads = a.hq + 2 * a.hkv;
   const int groups = (heads + 256 / D - 1) / (256 / D);   // warp passes of a token
   // One pass a warp while that leaves the launch within a few waves of the GPU (latency); beyond,
-  // four warps walk a whole token, so its positions and angles are read four times, not `groups` times.
+  // a block walks a whole token, so its angles are looked up once and not once per four passes.
   const int64_t blocks = static_cast<int64_t>(a.tokens) * ((groups + 3) / 4);
   const int passes = blocks <= 4096 ? 1 : (groups + 3) / 4;
   const dim3 grid(a.tokens, (groups + 4 * passes - 1) / (4 * passes));
-  kv8_store_kernel<D, kPairs, kPlain><<<grid, 128, 0, stream>>>(a, passes);
+  if (a.rot_dim == 0)
+    kv8_store_kernel<D, kNone><<<grid, 128, 0, stream>>>(a, passes);
+  else if (a.neox == 0)
+    kv8_store_kernel<D, kPairs><<<grid, 128, 0, stream>>>(a, passes);
+  else if (a.rot_dim % 16 == 0)
+    kv8_store_kernel<D, kHalves><<<grid, 128, 0, stream>>>(a, passes);
+  else
+    kv8_store_kernel<D, kOddHalves><<<grid, 128, 0, stream>>>(a, passes);
   return cudaGetLastError();
-}
-
-template <int D>
-cudaError_t launch_store(const Kv8StoreArgs& a, cudaStream_t stream) {
-  const int half = a.rot_dim / 2;
-  const bool pairs = a.neox == 0 && a.rot_dim > 0;
-  const bool axes = a.pos_rows == 3 && (a.section[1] > 0 || a.section[2] > 0);
-  const bool aligned = ((reinterpret_cast<uintptr_t>(a.cos_tab) | reinterpret_cast<uintptr_t>(a.sin_tab)) & 15) == 0;
-  const bool plain = !axes && aligned && half % 8 == 0;
-  if (pairs) return plain ? launch_store<D, true, true>(a, stream) : launch_store<D, true, false>(a, stream);
-  return plain ? launch_store<D, false, true>(a, stream) : launch_store<D, false, false>(a, stream);
 }
 
 }  // namespace
