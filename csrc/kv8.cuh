@@ -43,16 +43,18 @@ __device__ __forceinline__ int exponent_of(uint32_t amax_bits) {
   return max(kExpMin, min(kExpMax, e));
 }
 
-// Two e4m3 codes (low, high byte) as fp16 (exact).
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
-  uint32_t r;
-  asm("{\n .reg .b16 lo;\n cvt.u16.u32 lo, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(r) : "r"(two));
-  return r;
+// Four e4m3 codes (bytes 0 .. 3) as two fp16 pairs (exact).
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
 }
 
-__device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
-  const uint32_t h = e4m3x2_to_f16x2(two);
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+__device__ __forceinline__ float4 e4m3x4_to_f32(uint32_t four) {
+  uint32_t lo, hi;
+  e4m3x4_to_f16x4(four, lo, hi);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return make_float4(a.x, a.y, b.x, b.y);
 }
 
 // A block-table entry outside the cache reads the reserved padding page 0.

@@ -222,10 +222,12 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8ReadArgs a) {
     for (int k = 0; k < 2; ++k) {
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 t = e4m3x2_to_f32((w[2 * k + (j >> 1)] >> (16 * (j & 1))) & 0xffffu);
-        v[2 * j] = t.x * f;
-        v[2 * j + 1] = t.y * f;
+      for (int j = 0; j < 2; ++j) {
+        const float4 t = e4m3x4_to_f32(w[2 * k + j]);
+        v[4 * j] = t.x * f;
+        v[4 * j + 1] = t.y * f;
+        v[4 * j + 2] = t.z * f;
+        v[4 * j + 3] = t.w * f;
       }
       o[k] = pack8(v);
     }

@@ -248,6 +248,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == kWarps) {
     // ------------------------------------------------------------ producer
     int64_t t = 0;
+    int s = 0;                    // ring stage and phase
+    uint32_t ph = 1;
     bool ok = true;
     do {
       const Span sp(p, w.b);
@@ -258,10 +260,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int m = min(32, w.i1 - i);
         for (int j = 0; j < m; ++j, ++t) {
           const int page = __shfl_sync(0xffffffffu, mine, j);
-          const int s = static_cast<int>(t % kStages);
           bool go = true;
           if (lane == 0) {
-            if (t >= kStages) go = mbar_wait(&empty[s], static_cast<uint32_t>((t / kStages) & 1) ^ 1u, abort_flag, p.status);
+            if (t >= kStages) go = mbar_wait(&empty[s], ph, abort_flag, p.status);
             if (go) {
               const int r0 = (page * p.hkv + h) * kPage;
               uint8_t* dst = smem + s * S::kStage;
@@ -273,11 +274,9 @@ __global__ void __launch_bounds__(kThreads, 2)
               bulk_copy(de + kPage, p.v_exp + r0, kPage, &full[s]);
             }
           }
-          go = __shfl_sync(0xffffffffu, go, 0);
-          if (!go) {
-            ok = false;
-            break;
-          }
+          ok = __shfl_sync(0xffffffffu, go, 0);
+          if (!ok) break;
+          if (++s == kStages) s = 0, ph ^= 1;
         }
       }
     } while (ok && w.next(p));
@@ -291,7 +290,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   // -------------------------------------------------------------- consumers
   const int g = lane >> 2, t4 = lane & 3;
   const int lrow = warp * 16 + (lane & 15);                 // ldmatrix row of this lane
-  int64_t t = 0;
+  int s = 0;                      // ring stage and phase
+  uint32_t ph = 0;
   bool ok = true;
   bool more = true;
   while (more) {
@@ -341,9 +341,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       l[nt][0] = l[nt][1] = 0.f;
     }
 
-    for (int i = w.i0; i < w.i1; ++i, ++t) {
-      const int s = static_cast<int>(t % kStages);
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], static_cast<uint32_t>((t / kStages) & 1), abort_flag, p.status));
+    for (int i = w.i0; i < w.i1; ++i) {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], ph, abort_flag, p.status));
       if (!ok) continue;
       const uint32_t kt = smem_u32(smem + s * S::kStage), vt = kt + S::kTile;
       const int8_t* ex = reinterpret_cast<const int8_t*>(smem + S::kExp + s * 2 * kPage) + warp * 16;
@@ -360,8 +359,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         ldsm4(kt + swz<D>(lrow, c + (lane >> 4)), r);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint32_t a0 = e4m3x2_to_f16x2(r[2 * u]), a2 = e4m3x2_to_f16x2(r[2 * u] >> 16);
-          const uint32_t a1 = e4m3x2_to_f16x2(r[2 * u + 1]), a3 = e4m3x2_to_f16x2(r[2 * u + 1] >> 16);
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_to_f16x4(r[2 * u], a0, a2);
+          e4m3x4_to_f16x4(r[2 * u + 1], a1, a3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma(sc[nt], a0, a1, a2, a3, qf[nt][c + u][0], qf[nt][c + u][1]);
         }
@@ -440,15 +440,16 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           // bytes (key 2t: dims 2g, 2g+1; key 2t+1: the same) -> two keys of a dim side by side
-          const uint32_t lo = __byte_perm(r[2 * u] & keep[0], 0u, 0x3120), hi = __byte_perm(r[2 * u + 1] & keep[1], 0u, 0x3120);
-          const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(lo >> 16);
-          const uint32_t a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_to_f16x4(__byte_perm(r[2 * u] & keep[0], 0u, 0x3120), a0, a1);
+          e4m3x4_to_f16x4(__byte_perm(r[2 * u + 1] & keep[1], 0u, 0x3120), a2, a3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma(o[nt][c + u], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
+      if (++s == kStages) s = 0, ph ^= 1;
     }
 
     // join the four warps
