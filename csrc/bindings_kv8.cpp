@@ -1,6 +1,7 @@
 // torch bindings of the 8-bit paged KV cache (kv8_cache.cu, kv8_decode.cu, kv8_prefill.cu).  Every argument is
 // checked here, before anything is launched; a bad one raises with its name.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -43,13 +44,20 @@ Cache check_cache(const torch::Tensor& k, const torch::Tensor& v, const torch::T
   check_on(ke, k, "cache.k_exp");
   check_on(ve, k, "cache.v_exp");
   TORCH_CHECK(v.scalar_type() == k.scalar_type() && v.sizes() == k.sizes(), "cache.v must match cache.k");
-  const std::vector<int64_t> es{c.pages, c.hkv, 64};
-  TORCH_CHECK(ke.scalar_type() == at::kChar && ke.sizes() == es && ve.scalar_type() == at::kChar && ve.sizes() == es,
+  const int64_t es[3] = {c.pages, c.hkv, 64};
+  TORCH_CHECK(ke.scalar_type() == at::kChar && ke.sizes() == at::IntArrayRef(es) && ve.scalar_type() == at::kChar &&
+                  ve.sizes() == at::IntArrayRef(es),
               "cache.k_exp / v_exp must be int8 [pages, Hkv, 64]");
   TORCH_CHECK(k.is_contiguous() && v.is_contiguous() && ke.is_contiguous() && ve.is_contiguous(),
               "the cache's tensors must be contiguous");
   TORCH_CHECK(aligned16(k) && aligned16(v) && aligned16(ke) && aligned16(ve), "the cache's tensors must be 16-byte aligned");
   return c;
+}
+
+// Uninitialised tensor from the caching allocator (the dispatcher's share of torch::empty is a
+// third of a small call's host time).
+torch::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const torch::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
 }
 
 const int* int_ptr(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
@@ -104,7 +112,7 @@ torch::Tensor kv8_store(const torch::Tensor& qkv, const torch::Tensor& k, const 
                       aligned16(**w),
                   "q_norm / k_norm must be contiguous bf16 [head_dim]");
     }
-  torch::Tensor q = q_out.has_value() ? *q_out : torch::empty({T, hq * head_dim}, qkv.options());
+  torch::Tensor q = q_out.has_value() ? *q_out : empty({T, hq * head_dim}, at::kBFloat16, k);
   check_on(q, k, "out");
   check_rows(q, hq * head_dim, "out");
   TORCH_CHECK(q.size(0) == T, "out has " + num(q.size(0)) + " rows for " + num(T) + " tokens");
@@ -140,8 +148,7 @@ std::tuple<torch::Tensor, torch::Tensor> kv8_read(const torch::Tensor& k, const 
   omni::Kv8ReadArgs a{};
   a.slots = int_ptr(slots, k, "slots");
   TORCH_CHECK(slots.dim() == 1 && slots.numel() < (int64_t{1} << 31), "slots must be 1-D");
-  const auto opt = k.options().dtype(at::kBFloat16);
-  torch::Tensor ko = torch::empty({slots.numel(), c.hkv, c.d}, opt), vo = torch::empty({slots.numel(), c.hkv, c.d}, opt);
+  torch::Tensor ko = empty({slots.numel(), c.hkv, c.d}, at::kBFloat16, k), vo = empty({slots.numel(), c.hkv, c.d}, at::kBFloat16, k);
   a.count = static_cast<int>(slots.numel());
   a.hkv = static_cast<int>(c.hkv);
   a.head_dim = static_cast<int>(c.d);
@@ -187,7 +194,7 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
   } else {
     TORCH_CHECK(T == B, "decode takes one query row per request: " + num(T) + " rows, " + num(B) + " requests");
   }
-  torch::Tensor out = out_.has_value() ? *out_ : torch::empty({T, hq * head_dim}, q.options());
+  torch::Tensor out = out_.has_value() ? *out_ : empty({T, hq * head_dim}, at::kBFloat16, k);
   check_on(out, k, "out");
   check_rows(out, hq * head_dim, "out");
   TORCH_CHECK(out.size(0) == T, "out has " + num(out.size(0)) + " rows for " + num(T) + " query rows");
@@ -220,22 +227,21 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
   }
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   // scratch from the caching allocator, used on the current stream only
-  const auto f32 = k.options().dtype(at::kFloat);
   torch::Tensor scratch;
   if (!cu_q.has_value()) {
-    a.ctas = omni::kv8_decode_ctas(sms);
-    scratch = torch::empty({omni::kv8_decode_scratch_floats(a.ctas, static_cast<int>(hq / hkv), a.head_dim)}, f32);
+    a.ctas = omni::kv8_decode_ctas(sms, static_cast<int>(hq / hkv), a.head_dim);
+    scratch = empty({omni::kv8_decode_scratch_floats(a.ctas, static_cast<int>(hq / hkv), a.head_dim)}, at::kFloat, k);
     a.scratch = scratch.data_ptr<float>();
     check_launch(omni::kv8_decode(a, at::cuda::getCurrentCUDAStream()), "kv8_decode_attention");
   } else {
     a.splits = omni::kv8_prefill_splits(a, sms);
     if (a.splits > 1) {
-      scratch = torch::empty({omni::kv8_prefill_scratch_floats(a)}, f32);
+      scratch = empty({omni::kv8_prefill_scratch_floats(a)}, at::kFloat, k);
       a.scratch = scratch.data_ptr<float>();
     }
     torch::Tensor tiles;
     if (const int64_t bytes = omni::kv8_prefill_tile_bytes(a)) {
-      tiles = torch::empty({bytes}, k.options().dtype(at::kByte));
+      tiles = empty({bytes}, at::kByte, k);
       a.tiles = tiles.data_ptr();
     }
     check_launch(omni::kv8_prefill(a, at::cuda::getCurrentCUDAStream()), "kv8_prefill_attention");

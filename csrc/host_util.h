@@ -27,4 +27,22 @@ cudaError_t ensure_smem_attr(int bytes) {
   return e;
 }
 
+// A launch that may start while the one before it on the stream still runs (programmatic dependent
+// launch): every thread of its kernel calls grid_dep_wait() before it reads memory or exits.
+template <class... Args>
+cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int block, int smem, cudaStream_t stream,
+                             const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace omni

@@ -12,6 +12,7 @@
 //
 // Reference counterpart: the fp8 KV-cache option of SGLang's token-to-KV pool behind
 // sglang_omni/engines/ar/sglang_backend/server_args_builder.py:10-35 (kv_cache_dtype there).
+#include "host_util.h"
 #include "kv8.cuh"
 #include "omni_kernels.h"
 #include "pdl.cuh"
@@ -72,6 +73,7 @@ __global__ void __launch_bounds__(128, 8) kv8_store_kernel(const Kv8StoreArgs a,
   const int tok = blockIdx.x;
   const int head0 = (blockIdx.y * 4 + warp) * HW * passes + sub;
   const int half = a.rot_dim >> 1;
+  grid_dep_wait();
   const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.qkv) + static_cast<int64_t>(tok) * a.qkv_stride + l * 8;
   uint4 raw = head0 < heads ? *reinterpret_cast<const uint4*>(src + head0 * D) : make_uint4(0u, 0u, 0u, 0u);
   if (kRope != kNone && static_cast<int>(threadIdx.x) < half) {
@@ -202,6 +204,8 @@ __global__ void __launch_bounds__(128, 8) kv8_store_kernel(const Kv8StoreArgs a,
 template <int D>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8ReadArgs a) {
   constexpr int L = D / 16;
+  grid_dep_launch();
+  grid_dep_wait();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   const int64_t rows = static_cast<int64_t>(a.count) * a.hkv;
   const int64_t r = i / L;
@@ -251,14 +255,12 @@ cudaError_t launch_store(const Kv8StoreArgs& a, cudaStream_t stream) {
   const int passes = blocks <= 4096 ? 1 : (groups + 3) / 4;
   const dim3 grid(a.tokens, (groups + 4 * passes - 1) / (4 * passes));
   if (a.rot_dim == 0)
-    kv8_store_kernel<D, kNone><<<grid, 128, 0, stream>>>(a, passes);
-  else if (a.neox == 0)
-    kv8_store_kernel<D, kPairs><<<grid, 128, 0, stream>>>(a, passes);
-  else if (a.rot_dim % 16 == 0)
-    kv8_store_kernel<D, kHalves><<<grid, 128, 0, stream>>>(a, passes);
-  else
-    kv8_store_kernel<D, kOddHalves><<<grid, 128, 0, stream>>>(a, passes);
-  return cudaGetLastError();
+    return launch_dependent(kv8_store_kernel<D, kNone>, grid, 128, 0, stream, a, passes);
+  if (a.neox == 0)
+    return launch_dependent(kv8_store_kernel<D, kPairs>, grid, 128, 0, stream, a, passes);
+  if (a.rot_dim % 16 == 0)
+    return launch_dependent(kv8_store_kernel<D, kHalves>, grid, 128, 0, stream, a, passes);
+  return launch_dependent(kv8_store_kernel<D, kOddHalves>, grid, 128, 0, stream, a, passes);
 }
 
 }  // namespace
@@ -276,12 +278,10 @@ cudaError_t kv8_read(const Kv8ReadArgs& a, cudaStream_t stream) {
   const int64_t blocks = (threads + 255) / 256;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   if (a.head_dim == 128)
-    kv8_read_kernel<128><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
-  else if (a.head_dim == 64)
-    kv8_read_kernel<64><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
-  else
-    return cudaErrorInvalidValue;
-  return cudaGetLastError();
+    return launch_dependent(kv8_read_kernel<128>, dim3(static_cast<unsigned>(blocks)), 256, 0, stream, a);
+  if (a.head_dim == 64)
+    return launch_dependent(kv8_read_kernel<64>, dim3(static_cast<unsigned>(blocks)), 256, 0, stream, a);
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace omni

@@ -49,7 +49,14 @@ constexpr float kHead = 7.f;                    // weights are held times 2^7: b
 
 template <int D, int NT>
 struct Smem {
-  static constexpr int kStages = NT == 1 ? 5 : 4;   // two CTAs per SM in 227 KB
+#ifndef ST128
+#define ST128 3
+#define ST64 5
+#define CT128 3
+#define CT64 4
+#endif
+  static constexpr int kCtas = D == 128 ? (NT == 1 ? CT128 : 2) : (NT == 1 ? CT64 : 3);   // resident per SM
+  static constexpr int kStages = D == 128 ? (NT == 1 ? ST128 : 4) : ST64;
   static constexpr int kTile = kPage * D;       // bytes of a K or V tile
   static constexpr int kStage = 2 * kTile;
   static constexpr int kExp = kStages * kStage;                 // exponents: [stage][2][64]
@@ -211,7 +218,7 @@ __device__ __forceinline__ int swz(int r, int c) {
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
     kv8_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Params p) {
   using S = Smem<D, NT>;
   constexpr int kStages = S::kStages;
@@ -237,6 +244,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   __syncthreads();
   grid_dep_launch();   // the joining launch may set up; it waits for this grid before it reads
+  grid_dep_wait();
 
   const int R = p.hkv * p.head_groups;
   const int64_t W = count_tiles(p, 0, nullptr) * R;
@@ -513,17 +521,14 @@ template <int D, int NT>
 __global__ void __launch_bounds__(128) kv8_decode_join_kernel(const Params p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp;
-  if (row >= static_cast<int64_t>(p.batch) * p.hq) {
-    grid_dep_wait();
-    return;
-  }
+  grid_dep_wait();   // in every thread: the grid before may itself still wait for what wrote kv_lens
+  if (row >= static_cast<int64_t>(p.batch) * p.hq) return;
   const int b = static_cast<int>(row / p.hq), hq = static_cast<int>(row - static_cast<int64_t>(b) * p.hq);
   const int h = hq / p.group, in = hq - h * p.group, hg = in / (8 * NT), head = in - hg * 8 * NT;
   const int R = p.hkv * p.head_groups;
   int64_t before;
   const int64_t W = count_tiles(p, b, &before) * R;
   const int n = Span(p, b).tiles;
-  grid_dep_wait();                            // in every thread: what follows on the stream relies on it
   constexpr int PER = D / 32;
   __nv_bfloat16* out = p.out + static_cast<int64_t>(b) * p.out_stride + static_cast<int64_t>(hq) * D + lane * PER;
   float acc[PER];
@@ -587,24 +592,18 @@ cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p
   using S = Smem<D, NT>;
   cudaError_t e = ensure_smem_attr<kv8_decode_kernel<D, NT>>(S::kBytes);
   if (e != cudaSuccess) return e;
-  kv8_decode_kernel<D, NT><<<p.ctas, kThreads, S::kBytes, stream>>>(tk, tv, p);
-  e = cudaGetLastError();
+  e = launch_dependent(kv8_decode_kernel<D, NT>, dim3(p.ctas), kThreads, S::kBytes, stream, tk, tv, p);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.batch) * p.hq + 3) / 4));
-  cfg.blockDim = dim3(128);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv8_decode_join_kernel<D, NT>, p);
+  const int64_t rows = static_cast<int64_t>(p.batch) * p.hq;
+  return launch_dependent(kv8_decode_join_kernel<D, NT>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, p);
 }
 
 }  // namespace
 
-int kv8_decode_ctas(int sm_count) { return 2 * sm_count; }
+int kv8_decode_ctas(int sm_count, int group, int head_dim) {
+  return sm_count * (head_dim == 128 ? (group > 8 ? Smem<128, 2>::kCtas : Smem<128, 1>::kCtas)
+                                     : (group > 8 ? Smem<64, 2>::kCtas : Smem<64, 1>::kCtas));
+}
 
 int64_t kv8_decode_scratch_floats(int ctas, int group, int head_dim) {
   return 2 * static_cast<int64_t>(ctas) * (group > 8 ? 16 : 8) * (head_dim + 2);

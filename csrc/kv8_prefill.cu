@@ -320,6 +320,7 @@ struct Blocks {
 template <int D>
 __global__ void __launch_bounds__(kLoaders) kv8_expand_kernel(const Params p) {
   grid_dep_launch();
+  grid_dep_wait();
   const int req = blockIdx.y, h = blockIdx.z;
   const int n = p.cu_q[req + 1] - p.cu_q[req];
   const int kv_len = max(0, min(p.kv_lens[req], p.bt_pages * kPage));
@@ -730,35 +731,18 @@ __global__ void __launch_bounds__(128) kv8_prefill_join_kernel(const Params p) {
     *reinterpret_cast<__nv_bfloat162*>(out + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
 }
 
-// A launch that may start while the one before it on the stream still runs; its kernel waits.
-template <class... Args>
-cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int block, int smem, cudaStream_t stream, Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <int D>
 cudaError_t launch(const Params& p, int tiles, cudaStream_t stream) {
   const dim3 grid(tiles, p.hkv, p.splits);
   cudaError_t e;
   if (p.tiles != nullptr) {
     if ((e = ensure_smem_attr<kv8_prefill_kernel<D, true>>(Smem<D>::kBytes)) != cudaSuccess) return e;
-    kv8_expand_kernel<D><<<dim3(p.bt_pages, p.batch, p.hkv), kLoaders, 0, stream>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    e = launch_dependent(kv8_expand_kernel<D>, dim3(p.bt_pages, p.batch, p.hkv), kLoaders, 0, stream, p);
+    if (e != cudaSuccess) return e;
     e = launch_dependent(kv8_prefill_kernel<D, true>, grid, threads(true), Smem<D>::kBytes, stream, p);
   } else {
     if ((e = ensure_smem_attr<kv8_prefill_kernel<D, false>>(Smem<D>::kBytes)) != cudaSuccess) return e;
-    kv8_prefill_kernel<D, false><<<grid, threads(false), Smem<D>::kBytes, stream>>>(p);
-    e = cudaGetLastError();
+    e = launch_dependent(kv8_prefill_kernel<D, false>, grid, threads(false), Smem<D>::kBytes, stream, p);
   }
   if (e != cudaSuccess || p.splits == 1) return e;
   const int64_t rows = static_cast<int64_t>(p.q_rows) * p.hq;
