@@ -62,5 +62,71 @@ __device__ __forceinline__ int checked_page(int page, int num_pages) {
   return static_cast<unsigned>(page) >= static_cast<unsigned>(num_pages) ? 0 : page;
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Joins `count` partial softmax rows: ml(i) = (maximum in log2 units, sum), src(i) = D unnormalised
+// outputs, both relative to that maximum.  W warps of one block take the parts in turn and add their
+// sums in order, so the result does not depend on timing; the caller's block has 4 / W rows, and
+// `red` 4 * D floats of shared memory.  A part without a maximum is empty (sum 0, its outputs
+// unwritten) or carries a NaN.  Every thread of the block calls it; out is written by each row's first warp.
+template <int D, int W, class Ml, class Src>
+__device__ __forceinline__ void join_parts(int count, Ml ml, Src src, __nv_bfloat16* out, float* red) {
+  constexpr int PER = D / 32;
+  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) % W;
+  float mm = -INFINITY;
+  for (int i = lane; i < count; i += 32) mm = fmaxf(mm, ml(i).x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+  float acc[PER], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) acc[k] = 0.f;
+  for (int base = 0; base < count; base += 32) {
+    float2 v = make_float2(-INFINITY, 0.f);
+    if (base + lane < count) v = ml(base + lane);
+    const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : 1.f) : ex2(v.x - mm);
+    sum += v.y * f;
+    const int m = min(32, count - base);
+#pragma unroll 4
+    for (int i = w; i < m; i += W) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      float x[PER];
+#pragma unroll
+      for (int k = 0; k < PER; ++k) x[k] = 0.f;
+      if (fi != 0.f) {
+        const float* s = src(base + i) + lane * PER;
+        if constexpr (PER == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(s);
+          x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+        } else {
+          const float2 y = *reinterpret_cast<const float2*>(s);
+          x[0] = y.x, x[1] = y.y;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < PER; ++k) acc[k] += x[k] * fi;
+    }
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) red[(threadIdx.x >> 5) * D + lane * PER + k] = acc[k];
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int u = 1; u < W; ++u)
+#pragma unroll
+      for (int k = 0; k < PER; ++k) acc[k] += red[((threadIdx.x >> 5) + u) * D + lane * PER + k];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int k = 0; k < PER; k += 2)
+    *reinterpret_cast<__nv_bfloat162*>(out + lane * PER + k) = __floats2bfloat162_rn(acc[k] * inv, acc[k + 1] * inv);
+}
+
 }  // namespace kv8
 }  // namespace omni

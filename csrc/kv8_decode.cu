@@ -1,4 +1,5 @@
-// Decode attention over the 8-bit paged KV cache (form: kv8.cuh): one query token per request.
+// Decode attention over the 8-bit paged KV cache (form: kv8.cuh): one query token per request, or a few
+// tokens of chunks, each as a request of its own over the keys up to it.
 //
 //   o = sum_j p_j v_j,   p = softmax_j(q . k_j * scale) over the visible keys j
 //
@@ -76,6 +77,8 @@ struct Params {
   int64_t bt_stride;
   int bt_pages, num_pages;
   const int* kv_lens;
+  const int* cu_q;                              // nullptr, or chunks: query row b is a token of one of `requests`
+  int requests;
   int batch, hq, hkv, group, head_groups;       // head_groups: column tiles of 8 NT heads per KV head
   float scale;
   int window, sinks;
@@ -91,8 +94,21 @@ struct Params {
 struct Span {
   int kv, lo, sinks;      // keys [0, sinks) and [lo, kv)
   int sink_tiles, first, tiles;
+  int req;                // row of the block table
   __device__ Span(const Params& p, int b) {
-    kv = min(p.kv_lens[b], p.bt_pages * kPage);
+    if (p.cu_q == nullptr) {
+      req = b;
+      kv = min(p.kv_lens[b], p.bt_pages * kPage);
+    } else {              // the last request that starts at or before row b, and the keys up to its token
+      int lo_r = 0, hi_r = p.requests;
+      while (hi_r - lo_r > 1) {
+        const int mid = (lo_r + hi_r) >> 1;
+        if (p.cu_q[mid] <= b) lo_r = mid; else hi_r = mid;
+      }
+      req = lo_r;
+      const int after = p.cu_q[req + 1] - 1 - b;           // tokens of the chunk behind this one
+      kv = after < 0 ? 0 : min(p.kv_lens[req], p.bt_pages * kPage) - after;
+    }
     lo = p.window > 0 ? max(0, kv - p.window) : 0;
     sinks = min(p.sinks, lo);
     first = lo >> 6;
@@ -204,12 +220,6 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Byte offset of 16-byte chunk c of row r in a swizzled tile (128-byte swizzle for 128-byte rows,
 // 64-byte swizzle for 64-byte rows).
 template <int D>
@@ -262,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
     do {
       const Span sp(p, w.b);
       const int h = w.r / p.head_groups;
-      const int* row = p.block_table + static_cast<int64_t>(w.b) * p.bt_stride;
+      const int* row = p.block_table + static_cast<int64_t>(sp.req) * p.bt_stride;
       for (int i = w.i0; i < w.i1 && ok; i += 32) {
         const int mine = i + lane < w.i1 ? checked_page(row[sp.tile(i + lane)], p.num_pages) : 0;
         const int m = min(32, w.i1 - i);
@@ -516,49 +526,33 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
 }
 
 // Joins the partial sums of split pairs in the order of their CTAs, and writes zeros for requests
-// without a visible key.  One warp per (request, query head).
-template <int D, int NT>
+// without a visible key.  W warps per (request, query head).
+template <int D, int NT, int W>
 __global__ void __launch_bounds__(128) kv8_decode_join_kernel(const Params p) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp;
+  __shared__ float red[4 * D];
   grid_dep_wait();   // in every thread: the grid before may itself still wait for what wrote kv_lens
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / W) + (threadIdx.x >> 5) / W;
   if (row >= static_cast<int64_t>(p.batch) * p.hq) return;
   const int b = static_cast<int>(row / p.hq), hq = static_cast<int>(row - static_cast<int64_t>(b) * p.hq);
   const int h = hq / p.group, in = hq - h * p.group, hg = in / (8 * NT), head = in - hg * 8 * NT;
   const int R = p.hkv * p.head_groups;
   int64_t before;
-  const int64_t W = count_tiles(p, b, &before) * R;
+  const int64_t all = count_tiles(p, b, &before) * R;
   const int n = Span(p, b).tiles;
-  constexpr int PER = D / 32;
-  __nv_bfloat16* out = p.out + static_cast<int64_t>(b) * p.out_stride + static_cast<int64_t>(hq) * D + lane * PER;
-  float acc[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-  float ll = 0.f;
+  int64_t c0 = 0;
+  int count = 0;
   if (n > 0) {
-    const int64_t per = (W + p.ctas - 1) / p.ctas;
+    const int64_t per = (all + p.ctas - 1) / p.ctas;
     const int64_t x = before * R + static_cast<int64_t>(h * p.head_groups + hg) * n;
-    const int64_t c0 = x / per, c1 = (x + n - 1) / per;
-    if (c0 == c1) return;                     // written by its CTA
-    auto slot = [&](int64_t c) { return (c == c0 ? 2 * c + 1 : 2 * c) * 8 * NT + head; };
-    float mm = -INFINITY;
-    for (int64_t c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, p.part_ml[slot(c) * 2]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-#pragma unroll 4
-    for (int64_t c = c0; c <= c1; ++c) {
-      const float2 v = *reinterpret_cast<const float2*>(p.part_ml + slot(c) * 2);
-      const float f = v.x == -INFINITY ? 1.f : ex2(v.x - mm);
-      const float* src = p.part_o + slot(c) * D + lane * PER;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) acc[i] += src[i] * f;
-      ll += v.y * f;
-    }
+    c0 = x / per;
+    count = static_cast<int>((x + n - 1) / per - c0) + 1;
+    if (count == 1) return;                   // written by its CTA
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-#pragma unroll
-  for (int i = 0; i < PER; i += 2)
-    *reinterpret_cast<__nv_bfloat162*>(out + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
+  auto slot = [&](int i) { return (2 * (c0 + i) + (i == 0 ? 1 : 0)) * 8 * NT + head; };
+  join_parts<D, W>(
+      count, [&](int i) { return *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2); },
+      [&](int i) { return p.part_o + slot(i) * D; },
+      p.out + static_cast<int64_t>(b) * p.out_stride + static_cast<int64_t>(hq) * D, red);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -594,11 +588,20 @@ cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p
   if (e != cudaSuccess) return e;
   e = launch_dependent(kv8_decode_kernel<D, NT>, dim3(p.ctas), kThreads, S::kBytes, stream, tk, tv, p);
   if (e != cudaSuccess) return e;
+  // a row's parts: about ctas / pairs; four warps for many parts, one where there are few and many rows
   const int64_t rows = static_cast<int64_t>(p.batch) * p.hq;
-  return launch_dependent(kv8_decode_join_kernel<D, NT>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, p);
+  if (static_cast<int64_t>(p.batch) * p.hkv * p.head_groups * 4 <= p.ctas)
+    return launch_dependent(kv8_decode_join_kernel<D, NT, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, stream, p);
+  return launch_dependent(kv8_decode_join_kernel<D, NT, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, p);
 }
 
 }  // namespace
+
+#ifndef FEWT
+#define FEWT 16
+#endif
+// Chunks of few tokens read the context once per token, mostly out of L2.
+bool kv8_few_tokens(const Kv8AttnArgs& a) { return a.q_rows <= FEWT; }
 
 int kv8_decode_ctas(int sm_count, int group, int head_dim) {
   return sm_count * (head_dim == 128 ? (group > 8 ? Smem<128, 2>::kCtas : Smem<128, 1>::kCtas)
@@ -610,7 +613,7 @@ int64_t kv8_decode_scratch_floats(int ctas, int group, int head_dim) {
 }
 
 cudaError_t kv8_decode(const Kv8AttnArgs& a, cudaStream_t stream) {
-  if (a.batch == 0) return cudaSuccess;
+  if (a.q_rows == 0) return cudaSuccess;
   CUtensorMap tk, tv;
   const int64_t rows = static_cast<int64_t>(a.num_pages) * a.hkv * kPage;
   if (!encode(&tk, a.k, a.head_dim, rows) || !encode(&tv, a.v, a.head_dim, rows)) return cudaErrorInvalidValue;
@@ -624,7 +627,9 @@ cudaError_t kv8_decode(const Kv8AttnArgs& a, cudaStream_t stream) {
   p.bt_pages = a.bt_pages;
   p.num_pages = a.num_pages;
   p.kv_lens = a.kv_lens;
-  p.batch = a.batch;
+  p.cu_q = a.cu_q;
+  p.requests = a.batch;
+  p.batch = a.q_rows;
   p.hq = a.hq;
   p.hkv = a.hkv;
   p.group = a.hq / a.hkv;

@@ -153,12 +153,6 @@ __device__ __forceinline__ uint64_t umma_desc_mn(uint32_t smem_addr, uint32_t lb
   return d;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Two fp32 lanes per instruction, and a maximum of three: the softmax's arithmetic is bound by issue slots.
 __device__ __forceinline__ uint64_t f32x2(float a, float b) {
   uint64_t r;
@@ -695,40 +689,20 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
   }
 }
 
-// Joins the splits' partial outputs of each row in order.  One warp per (token, query head); a
+// Joins the splits' partial outputs of each row in order.  W warps per (token, query head); a
 // token that no request names keeps what the output held.
-template <int D>
+template <int D, int W>
 __global__ void __launch_bounds__(128) kv8_prefill_join_kernel(const Params p) {
+  __shared__ float red[4 * D];
   grid_dep_wait();
   const int64_t rows = static_cast<int64_t>(p.q_rows) * p.hq;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / W) + (threadIdx.x >> 5) / W;
   if (row >= rows) return;
   const int64_t tok = row / p.hq;
   if (tok >= p.cu_q[p.batch]) return;
-  constexpr int PER = D / 32;
-  float mm = -INFINITY;
-  for (int z = lane; z < p.splits; z += 32) mm = fmaxf(mm, p.part_ml[z * rows + row].x);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-  float acc[PER], ll = 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int z = 0; z < p.splits; ++z) {
-    const float2 v = p.part_ml[z * rows + row];
-    if (v.y == 0.f) continue;                          // a split without a visible key
-    const float f = v.x == -INFINITY ? 1.f : ex2(v.x - mm);   // without a maximum: a NaN to pass on
-    const float* src = p.part_o + (z * rows + row) * D + lane * PER;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] += src[i] * f;
-    ll += v.y * f;
-  }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  __nv_bfloat16* out = p.out + tok * p.out_stride + (row - tok * p.hq) * D + lane * PER;
-#pragma unroll
-  for (int i = 0; i < PER; i += 2)
-    *reinterpret_cast<__nv_bfloat162*>(out + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
+  join_parts<D, W>(
+      p.splits, [&](int z) { return p.part_ml[z * rows + row]; }, [&](int z) { return p.part_o + (z * rows + row) * D; },
+      p.out + tok * p.out_stride + (row - tok * p.hq) * D, red);
 }
 
 template <int D>
@@ -746,7 +720,8 @@ cudaError_t launch(const Params& p, int tiles, cudaStream_t stream) {
   }
   if (e != cudaSuccess || p.splits == 1) return e;
   const int64_t rows = static_cast<int64_t>(p.q_rows) * p.hq;
-  return launch_dependent(kv8_prefill_join_kernel<D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, p);
+  if (p.splits > 8) return launch_dependent(kv8_prefill_join_kernel<D, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, stream, p);
+  return launch_dependent(kv8_prefill_join_kernel<D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, p);
 }
 
 int64_t row_tiles(int64_t q_rows, int batch, int group) {

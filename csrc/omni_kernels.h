@@ -253,7 +253,8 @@ int64_t kv8_prefill_tile_bytes(const Kv8AttnArgs& a);   // after `splits` is set
 cudaError_t kv8_prefill(const Kv8AttnArgs& a, cudaStream_t stream);
 int kv8_decode_ctas(int sm_count, int group, int head_dim);
 int64_t kv8_decode_scratch_floats(int ctas, int group, int head_dim);
-cudaError_t kv8_decode(const Kv8AttnArgs& a, cudaStream_t stream);
+cudaError_t kv8_decode(const Kv8AttnArgs& a, cudaStream_t stream);   // cu_q: each row its own request
+bool kv8_few_tokens(const Kv8AttnArgs& a);   // chunks that kv8_decode takes
 
 struct MoeRouteArgs {
   const float* logits;     // [tokens, experts] router logits (fp32)
