@@ -234,15 +234,15 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
     a.scratch = scratch.data_ptr<float>();
     check_launch(omni::kv8_decode(a, at::cuda::getCurrentCUDAStream()), "kv8_decode_attention");
   } else {
-    a.splits = omni::kv8_prefill_splits(a, sms);
-    if (a.splits > 1) {
-      scratch = empty({omni::kv8_prefill_scratch_floats(a)}, at::kFloat, k);
-      a.scratch = scratch.data_ptr<float>();
-    }
     torch::Tensor tiles;
     if (const int64_t bytes = omni::kv8_prefill_tile_bytes(a)) {
       tiles = empty({bytes}, at::kByte, k);
       a.tiles = tiles.data_ptr();
+    }
+    a.splits = omni::kv8_prefill_splits(a, sms);
+    if (a.splits > 1) {
+      scratch = empty({omni::kv8_prefill_scratch_floats(a)}, at::kFloat, k);
+      a.scratch = scratch.data_ptr<float>();
     }
     check_launch(omni::kv8_prefill(a, at::cuda::getCurrentCUDAStream()), "kv8_prefill_attention");
   }

@@ -597,11 +597,14 @@ cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p
 
 }  // namespace
 
-#ifndef FEWT
-#define FEWT 16
-#endif
-// Chunks of few tokens read the context once per token, mostly out of L2.
-bool kv8_few_tokens(const Kv8AttnArgs& a) { return a.q_rows <= FEWT; }
+// Chunks of few tokens: the decode kernel reads the context once per token (mostly out of L2), the chunk
+// kernel once, but expands it.  Microseconds, decode / chunk kernel, 32 / 4 heads of 128: 4 tokens on
+// 3000 keys 14 / 17, on 16,000 22 / 22, on 100,000 66 / 67; 8 tokens on 3000 keys 16 / 18, on
+// 100,000 118 / 69; 32 / 8 heads of 64: 4 tokens 13 / 12, 23 / 21, 84 / 87.
+bool kv8_few_tokens(const Kv8AttnArgs& a) {
+  const int64_t rows = a.q_rows, requests = a.batch;
+  return (rows <= 4 * requests && rows <= 512) || (rows <= 8 * requests && rows <= 64 && a.bt_pages <= 64);
+}
 
 int kv8_decode_ctas(int sm_count, int group, int head_dim) {
   return sm_count * (head_dim == 128 ? (group > 8 ? Smem<128, 2>::kCtas : Smem<128, 1>::kCtas)

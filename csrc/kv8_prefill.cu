@@ -42,8 +42,13 @@ using namespace kv8;
 constexpr int kRows = 128;                 // rows of a query tile
 constexpr int kBN = kPage;                 // keys of a block
 constexpr int kStages = 5;
-constexpr int kLoaders = 128;
-constexpr int threads(bool expanded) { return 256 + (expanded ? 32 : kLoaders) + 32; }
+constexpr int kExpandThreads = 128;
+// Two query tiles and one loader warp where the tiles come expanded; one query tile and eight loader
+// warps where the loaders expand them (the few rows of such a launch do not fill a second tile, and four
+// loader warps took 3000 cycles a block, twice the softmax's time).
+constexpr int tiles_of(bool expanded) { return expanded ? 2 : 1; }
+constexpr int load_warps(bool expanded) { return expanded ? 1 : 8; }
+constexpr int threads(bool expanded) { return 32 * (4 * tiles_of(expanded) + load_warps(expanded) + 1); }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.0f;             // log2 units
 constexpr int kTmemCols = 512;             // S/P: tile x buffer x 64, O: tile x D
@@ -233,15 +238,22 @@ __device__ __forceinline__ uint2 expand4(uint32_t w, const RowScale& s) {
 template <int N>
 struct Share {
   uint4 k[N], v[N];
-  uint32_t ke, ve;
+  uint32_t ke, ve;      // one byte per row
 };
 
-template <int D>
+template <int N>
+__device__ __forceinline__ uint32_t load_bytes(const int8_t* p) {
+  if constexpr (N == 4) return __ldg(reinterpret_cast<const uint32_t*>(p));
+  if constexpr (N == 2) return __ldg(reinterpret_cast<const uint16_t*>(p));
+  return __ldg(reinterpret_cast<const uint8_t*>(p));
+}
+
+template <int D, int TH>
 struct Part {
   static constexpr int CH = D / 16;              // 16-code chunks of a row
-  static constexpr int N = kBN * CH / kLoaders;  // rows per thread
+  static constexpr int N = kBN * CH / TH;        // rows per thread
   Share<N> x;
-  // Thread `tid` of 128 reads its share of the block whose first row is row0.
+  // Thread `tid` of TH reads its share of the block whose first row is row0.
   __device__ __forceinline__ void fetch(const Params& p, int64_t row0, int tid) {
     row0 += tid / CH * N;
     const uint8_t* k = p.k + row0 * D + tid % CH * 16;
@@ -251,13 +263,8 @@ struct Part {
       x.k[i] = __ldg(reinterpret_cast<const uint4*>(k + i * D));
       x.v[i] = __ldg(reinterpret_cast<const uint4*>(v + i * D));
     }
-    if constexpr (N == 4) {
-      x.ke = __ldg(reinterpret_cast<const uint32_t*>(p.k_exp + row0));
-      x.ve = __ldg(reinterpret_cast<const uint32_t*>(p.v_exp + row0));
-    } else {
-      x.ke = __ldg(reinterpret_cast<const uint16_t*>(p.k_exp + row0));
-      x.ve = __ldg(reinterpret_cast<const uint16_t*>(p.v_exp + row0));
-    }
+    x.ke = load_bytes<N>(p.k_exp + row0);
+    x.ve = load_bytes<N>(p.v_exp + row0);
   }
   // Expands it into the block's K and V tiles (the tensor core's swizzled layout); rows from `left`
   // on lie past the context: their values become zeros (their scores are masked).
@@ -312,7 +319,7 @@ struct Blocks {
 // Expands every block that a request's new tokens see, once, into `tiles` (K tile, V tile of each
 // [request][page][KV head], as they will lie in shared memory).
 template <int D>
-__global__ void __launch_bounds__(kLoaders) kv8_expand_kernel(const Params p) {
+__global__ void __launch_bounds__(kExpandThreads) kv8_expand_kernel(const Params p) {
   grid_dep_launch();
   grid_dep_wait();
   const int req = blockIdx.y, h = blockIdx.z;
@@ -323,18 +330,18 @@ __global__ void __launch_bounds__(kLoaders) kv8_expand_kernel(const Params p) {
   if (static_cast<int>(blockIdx.x) >= bl.count) return;
   const int i = bl.at(blockIdx.x);
   const int page = checked_page(p.block_table[static_cast<int64_t>(req) * p.bt_stride + i], p.num_pages);
-  Part<D> part;
+  Part<D, kExpandThreads> part;
   part.fetch(p, (static_cast<int64_t>(page) * p.hkv + h) * kPage, threadIdx.x);
   uint8_t* dst = p.tiles + ((static_cast<int64_t>(req) * p.bt_pages + i) * p.hkv + h) * (2 * Smem<D>::kKBytes);
   part.store(dst, dst + Smem<D>::kKBytes, kv_len - i * kPage, threadIdx.x);
 }
 
-// kExpanded: the K / V tiles come ready from kv8_expand_kernel by bulk copies, one loader warp.
+// kExpanded: the K / V tiles come ready from kv8_expand_kernel by bulk copies.
 template <int D, bool kExpanded>
 __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(const Params p) {
   using S = Smem<D>;
-  constexpr int kLoadWarps = kExpanded ? 1 : kLoaders / 32;
-  constexpr int kMmaWarp = 8 + kLoadWarps;
+  constexpr int kTiles = tiles_of(kExpanded), kLoadWarps = load_warps(kExpanded);
+  constexpr int kLoad0 = 4 * kTiles, kMmaWarp = kLoad0 + kLoadWarps;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
@@ -355,7 +362,7 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
   // row tile of this CTA, the last ones (with the most keys) first
   int req = -1, tok0 = 0;
   {
-    const int step = 2 * p.tpt;
+    const int step = kTiles * p.tpt;
     int total = 0;
     for (int base = 0; base < p.batch; base += 32) {
       int n = 0;
@@ -388,8 +395,8 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
   const int q_len = min(p.cu_q[req + 1], p.q_rows) - q_begin;   // cu_q never names rows past q
   const int kv_len = max(0, min(p.kv_lens[req], p.bt_pages * kPage));
   const int past = kv_len - (p.cu_q[req + 1] - q_begin);        // keys before the chunk's first query
-  const int tiles = q_len - tok0 > p.tpt ? 2 : 1;
-  const Blocks bl(p, kv_len, past + tok0, min(q_len - tok0, 2 * p.tpt));
+  const int tiles = kTiles == 2 && q_len - tok0 > p.tpt ? 2 : 1;
+  const Blocks bl(p, kv_len, past + tok0, min(q_len - tok0, kTiles * p.tpt));
   const int j0 = static_cast<int>(static_cast<int64_t>(bl.count) * z / p.splits);
   const int nb = static_cast<int>(static_cast<int64_t>(bl.count) * (z + 1) / p.splits) - j0;
   auto block_of = [&](int j) { return bl.at(j0 + j); };
@@ -423,7 +430,7 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
   auto s_col = [](int t, int b) -> uint32_t { return static_cast<uint32_t>(t * 2 + b) * 64u; };
   auto o_col = [](int t) -> uint32_t { return 256u + static_cast<uint32_t>(t) * D; };
 
-  if (warp >= 8 && warp < kMmaWarp) {
+  if (warp >= kLoad0 && warp < kMmaWarp) {
     // ------------------------------------------------------------ loaders
     int stage = 0;
     uint32_t phase = 1;                     // the first round finds the ring empty
@@ -443,18 +450,19 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
       }
       __syncwarp();
     } else {
-      const int tid = threadIdx.x - 256;
+      constexpr int TH = 32 * kLoadWarps;
+      const int tid = threadIdx.x - 32 * kLoad0;
       const int* table = p.block_table + static_cast<int64_t>(req) * p.bt_stride;
       auto page_of = [&](int j) { return j < nb ? checked_page(table[block_of(j)], p.num_pages) : 0; };
-      auto fetch = [&](int j, int page, Part<D>& x) {
+      auto fetch = [&](int j, int page, Part<D, TH>& x) {
         if (j < nb) x.fetch(p, (static_cast<int64_t>(page) * p.hkv + h) * kPage, tid);
       };
-      Part<D> buf[3];                       // blocks j, j + 1, j + 2
+      Part<D, TH> buf[3];                       // blocks j, j + 1, j + 2
       bool ok = true;
       int page = page_of(2);
       fetch(0, page_of(0), buf[0]);
       fetch(1, page_of(1), buf[1]);
-      auto put = [&](int j, Part<D>& cur, Part<D>& far) {
+      auto put = [&](int j, Part<D, TH>& cur, Part<D, TH>& far) {
         fetch(j + 2, page, far);
         page = page_of(j + 3);
         if (j >= kStages) ok = warp_wait(&kv_empty[stage], phase, abort_flag, p.status, 41);
@@ -711,7 +719,7 @@ cudaError_t launch(const Params& p, int tiles, cudaStream_t stream) {
   cudaError_t e;
   if (p.tiles != nullptr) {
     if ((e = ensure_smem_attr<kv8_prefill_kernel<D, true>>(Smem<D>::kBytes)) != cudaSuccess) return e;
-    e = launch_dependent(kv8_expand_kernel<D>, dim3(p.bt_pages, p.batch, p.hkv), kLoaders, 0, stream, p);
+    e = launch_dependent(kv8_expand_kernel<D>, dim3(p.bt_pages, p.batch, p.hkv), kExpandThreads, 0, stream, p);
     if (e != cudaSuccess) return e;
     e = launch_dependent(kv8_prefill_kernel<D, true>, grid, threads(true), Smem<D>::kBytes, stream, p);
   } else {
@@ -724,26 +732,29 @@ cudaError_t launch(const Params& p, int tiles, cudaStream_t stream) {
   return launch_dependent(kv8_prefill_join_kernel<D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, p);
 }
 
-int64_t row_tiles(int64_t q_rows, int batch, int group) {
-  const int64_t step = 2 * (kRows / group);
+int64_t row_tiles(int64_t q_rows, int batch, int group, bool expanded) {
+  const int64_t step = tiles_of(expanded) * (kRows / group);
   return std::min(q_rows, q_rows / step + batch);     // each request ends in at most one partial tile
 }
 
 }  // namespace
 
-// Splits of the key blocks: as many as keep the launch within one CTA per SM, one where the row
-// tiles alone fill the GPU.
-int kv8_prefill_splits(const Kv8AttnArgs& a, int sm_count) {
-  const int64_t base = row_tiles(a.q_rows, a.batch, a.hq / a.hkv) * a.hkv;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count / std::max<int64_t>(1, base), a.bt_pages)));
-}
-
-// Bytes of the expanded tiles, 0 where the blocks are expanded in the attention kernel itself.
+// Bytes of the expanded tiles; 0 where the blocks are expanded in the attention kernel itself.  A launch
+// of its own costs each block a write and reads of the expanded form, but once for all row tiles.
+// One request, 32 / 4 heads of 128, microseconds with / without it: 64 new tokens (2 pairs of row tiles) on
+// 3000 keys 26 / 22, on 16,000 48 / 50, on 100,000 189 / 276; 128 tokens 31 / 28, 63 / 75, 272 / 460.
 int64_t kv8_prefill_tile_bytes(const Kv8AttnArgs& a) {
   const int64_t step = 2 * (kRows / (a.hq / a.hkv));
   const int64_t bytes = static_cast<int64_t>(a.batch) * a.bt_pages * a.hkv * kPage * a.head_dim * 4;
-  if (a.q_rows < 2 * step * a.batch || a.splits > 1 || bytes > (int64_t{1} << 31) || a.batch > 65535) return 0;
+  if (a.q_rows < 2 * step * a.batch || bytes > (int64_t{1} << 31) || a.batch > 65535 || a.hkv > 65535) return 0;
   return bytes;
+}
+
+// Splits of the key blocks: as many as keep the launch within one CTA per SM, one where the row
+// tiles alone fill the GPU.
+int kv8_prefill_splits(const Kv8AttnArgs& a, int sm_count) {
+  const int64_t base = row_tiles(a.q_rows, a.batch, a.hq / a.hkv, a.tiles != nullptr) * a.hkv;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count / std::max<int64_t>(1, base), a.bt_pages)));
 }
 
 int64_t kv8_prefill_scratch_floats(const Kv8AttnArgs& a) {
@@ -783,7 +794,7 @@ cudaError_t kv8_prefill(const Kv8AttnArgs& a, cudaStream_t stream) {
   p.part_ml = reinterpret_cast<float2*>(a.scratch + static_cast<int64_t>(a.splits) * a.q_rows * a.hq * a.head_dim);
   p.tiles = static_cast<uint8_t*>(a.tiles);
   p.status = a.status;
-  const int64_t tiles = row_tiles(a.q_rows, a.batch, group);
+  const int64_t tiles = row_tiles(a.q_rows, a.batch, group, a.tiles != nullptr);
   if (tiles > 0x7fffffff || a.hkv > 65535) return cudaErrorInvalidValue;
   if (a.head_dim == 128) return launch<128>(p, static_cast<int>(tiles), stream);
   if (a.head_dim == 64) return launch<64>(p, static_cast<int>(tiles), stream);

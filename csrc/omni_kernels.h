@@ -247,9 +247,9 @@ struct Kv8AttnArgs {
   void* tiles;             // chunk: expanded key blocks (kv8_prefill_tile_bytes), or nullptr
   int* status;             // bounded-wait status word, may be nullptr
 };
-int kv8_prefill_splits(const Kv8AttnArgs& a, int sm_count);
-int64_t kv8_prefill_scratch_floats(const Kv8AttnArgs& a);
-int64_t kv8_prefill_tile_bytes(const Kv8AttnArgs& a);   // after `splits` is set
+int64_t kv8_prefill_tile_bytes(const Kv8AttnArgs& a);
+int kv8_prefill_splits(const Kv8AttnArgs& a, int sm_count);   // after `tiles` is set
+int64_t kv8_prefill_scratch_floats(const Kv8AttnArgs& a);     // after `splits` is set
 cudaError_t kv8_prefill(const Kv8AttnArgs& a, cudaStream_t stream);
 int kv8_decode_ctas(int sm_count, int group, int head_dim);
 int64_t kv8_decode_scratch_floats(int ctas, int group, int head_dim);
