@@ -359,38 +359,46 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
   grid_dep_launch();
   grid_dep_wait();
 
-  // row tile of this CTA, the last ones (with the most keys) first
+  // Row tile and KV head of this CTA.  The grid hands CTAs out in order, and the last to start should be
+  // short: requests by falling context (up to 32 of them; by position in the batch beyond), each
+  // request's tiles from its last, and all KV heads of a tile side by side.
   int req = -1, tok0 = 0;
+  const int h = static_cast<int>(blockIdx.x % p.hkv), z = blockIdx.y;
   {
     const int step = kTiles * p.tpt;
-    int total = 0;
-    for (int base = 0; base < p.batch; base += 32) {
-      int n = 0;
-      if (base + lane < p.batch) n = (max(0, p.cu_q[base + lane + 1] - p.cu_q[base + lane]) + step - 1) / step;
-      total += __reduce_add_sync(0xffffffffu, n);
-    }
-    const int x = total - 1 - static_cast<int>(blockIdx.x);
-    if (x < 0) return;
+    const int x = static_cast<int>(blockIdx.x / p.hkv);
     int cum = 0;
     for (int base = 0; base < p.batch && req < 0; base += 32) {
-      int n = 0;
-      if (base + lane < p.batch) n = (max(0, p.cu_q[base + lane + 1] - p.cu_q[base + lane]) + step - 1) / step;
-      int inc = n;
+      const int r = base + lane;
+      const int n = r < p.batch ? (max(0, p.cu_q[r + 1] - p.cu_q[r]) + step - 1) / step : 0;
+      int before = 0, all = 0;
+      if (p.batch <= 32) {
+        const int key = r < p.batch ? p.kv_lens[r] : 0;
+        for (int i = 0; i < p.batch; ++i) {
+          const int ki = __shfl_sync(0xffffffffu, key, i), ni = __shfl_sync(0xffffffffu, n, i);
+          if (ki > key || (ki == key && i < lane)) before += ni;
+        }
+      } else {
+        before = n;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, inc, d);
-        if (lane >= d) inc += up;
+        for (int d = 1; d < 32; d <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, before, d);
+          if (lane >= d) before += up;
+        }
+        all = __shfl_sync(0xffffffffu, before, 31);
+        before -= n;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, cum + inc > x);
-      if (past != 0) {
-        const int at = __ffs(past) - 1;
+      const int in = x - cum - before;
+      const unsigned mine = __ballot_sync(0xffffffffu, in >= 0 && in < n);
+      if (mine != 0) {
+        const int at = __ffs(mine) - 1;
         req = base + at;
-        tok0 = (x - cum - __shfl_sync(0xffffffffu, inc - n, at)) * step;
+        tok0 = __shfl_sync(0xffffffffu, (n - 1 - in) * step, at);
       }
-      cum += __shfl_sync(0xffffffffu, inc, 31);
+      cum += all;
     }
+    if (req < 0) return;
   }
-  const int h = blockIdx.y, z = blockIdx.z;
   const int q_begin = max(0, p.cu_q[req]);
   const int q_len = min(p.cu_q[req + 1], p.q_rows) - q_begin;   // cu_q never names rows past q
   const int kv_len = max(0, min(p.kv_lens[req], p.bt_pages * kPage));
@@ -714,8 +722,8 @@ __global__ void __launch_bounds__(128) kv8_prefill_join_kernel(const Params p) {
 }
 
 template <int D>
-cudaError_t launch(const Params& p, int tiles, cudaStream_t stream) {
-  const dim3 grid(tiles, p.hkv, p.splits);
+cudaError_t launch(const Params& p, int64_t tiles, cudaStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(tiles), p.splits);
   cudaError_t e;
   if (p.tiles != nullptr) {
     if ((e = ensure_smem_attr<kv8_prefill_kernel<D, true>>(Smem<D>::kBytes)) != cudaSuccess) return e;
@@ -794,10 +802,10 @@ cudaError_t kv8_prefill(const Kv8AttnArgs& a, cudaStream_t stream) {
   p.part_ml = reinterpret_cast<float2*>(a.scratch + static_cast<int64_t>(a.splits) * a.q_rows * a.hq * a.head_dim);
   p.tiles = static_cast<uint8_t*>(a.tiles);
   p.status = a.status;
-  const int64_t tiles = row_tiles(a.q_rows, a.batch, group, a.tiles != nullptr);
-  if (tiles > 0x7fffffff || a.hkv > 65535) return cudaErrorInvalidValue;
-  if (a.head_dim == 128) return launch<128>(p, static_cast<int>(tiles), stream);
-  if (a.head_dim == 64) return launch<64>(p, static_cast<int>(tiles), stream);
+  const int64_t tiles = row_tiles(a.q_rows, a.batch, group, a.tiles != nullptr) * a.hkv;
+  if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
+  if (a.head_dim == 128) return launch<128>(p, tiles, stream);
+  if (a.head_dim == 64) return launch<64>(p, tiles, stream);
   return cudaErrorInvalidValue;
 }
 
