@@ -2,6 +2,7 @@
 
     python examples/hf_llm_engine.py --model /models/Meta-Llama-3-8B-Instruct --prompt "Hello"
     python examples/hf_llm_engine.py --tiny          # a small random Llama, no checkpoint needed (CPU)
+    python examples/hf_llm_engine.py --tiny --window 16 --kv-format e4m3   # a sliding-window model, 8-bit KV cache
 
 ``create_ar_engine`` accepts the transformers model itself (as the reference's generic AR engine
 factory does) and moves its weights into the shared decoder, so generation runs on the paged KV
@@ -18,6 +19,9 @@ def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--model", help="checkpoint directory of a Llama / Mistral / Qwen2 / Qwen3 / Qwen3-MoE model")
     ap.add_argument("--tiny", action="store_true", help="a small random Llama instead of a checkpoint")
+    ap.add_argument("--window", type=int, default=0, help="with --tiny: a sliding window (a random Mistral)")
+    ap.add_argument("--kv-format", default="native", choices=["native", "e4m3"],
+                    help="e4m3: the KV cache in 8 bits (half the bytes; needed for sliding-window models)")
     ap.add_argument("--prompt", default="Hello")
     ap.add_argument("--max-new-tokens", type=int, default=16)
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
@@ -30,9 +34,16 @@ def main():
     from sglang_omni_b200.sampling_params import SamplingParams
 
     if a.tiny:
-        cfg = transformers.LlamaConfig(vocab_size=512, hidden_size=128, intermediate_size=256, num_hidden_layers=2,
-                                       num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=512)
-        cfg.architectures = ["LlamaForCausalLM"]
+        sizes = dict(vocab_size=512, hidden_size=128, intermediate_size=256, num_hidden_layers=2,
+                     num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=512)
+        if a.kv_format != "native":
+            sizes["head_dim"] = 64              # the 8-bit cache takes head dims 64 and 128
+        if a.window:
+            cfg = transformers.MistralConfig(**sizes, sliding_window=a.window)
+            cfg.architectures = ["MistralForCausalLM"]
+        else:
+            cfg = transformers.LlamaConfig(**sizes)
+            cfg.architectures = ["LlamaForCausalLM"]
         torch.manual_seed(0)
         hf = transformers.AutoModelForCausalLM.from_config(cfg).float().eval()
         ids = [1] + [ord(c) % 512 for c in a.prompt]
@@ -43,7 +54,8 @@ def main():
         ids = tok.apply_chat_template([{"role": "user", "content": a.prompt}], add_generation_prompt=True)
         decode = lambda toks: tok.decode(toks, skip_special_tokens=True)  # noqa: E731
 
-    engine = create_ar_engine(hf, max_seq_len=1024, device=a.device, max_batch=8, use_graphs=a.device != "cpu")
+    engine = create_ar_engine(hf, max_seq_len=1024, device=a.device, max_batch=8, use_graphs=a.device != "cpu",
+                              kv_format=a.kv_format)
     del hf
 
     async def run():

@@ -1,5 +1,9 @@
 """Paged KV pool: one tensor [layers, 2, pages, Hkv, 64, D] and a page allocator.
 
+``kv_format="e4m3"`` holds the keys and values in 8 bits instead (``ops.KV8Layers``: e4m3 codes and
+one power-of-two exponent per token and head), about half the bytes per token; the decoder then
+writes and reads it with the ``ops.kv8_*`` operators, which also carry sliding windows.
+
 Page 0 is reserved as the padding page of CUDA-graph decode buckets.
 The allocator is the native ``_runtime.PageAllocator`` when built, else a
 Python free list with the same interface.
@@ -18,12 +22,21 @@ from __future__ import annotations
 
 import torch
 
+from ...ops.kv8 import FORMATS, KV8Layers
+
 try:
     from ... import _runtime as _rt
 except ImportError:  # pragma: no cover
     _rt = None
 
 PAGE = 64
+
+
+def check_kv_format(kv_format: str) -> str:
+    """``native`` (the model's dtype) or one of the 8-bit formats."""
+    if kv_format != "native" and kv_format not in FORMATS:
+        raise ValueError(f"kv_format {kv_format!r} is not one of {('native', *FORMATS)}")
+    return kv_format
 
 
 class _PyAllocator:
@@ -56,11 +69,18 @@ class _PyAllocator:
 
 class KVPool:
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int, device,
-                 dtype=torch.bfloat16):
+                 dtype=torch.bfloat16, kv_format: str = "native"):
         self.device = torch.device(device)
         self.num_layers = num_layers
         self.num_pages = num_pages
-        self.kv = torch.zeros(num_layers, 2, num_pages, num_kv_heads, PAGE, head_dim, dtype=dtype, device=self.device)
+        self.kv_format = check_kv_format(kv_format)
+        if kv_format == "native":
+            self.kv = torch.zeros(num_layers, 2, num_pages, num_kv_heads, PAGE, head_dim, dtype=dtype,
+                                  device=self.device)
+        else:
+            if head_dim not in (64, 128):
+                raise ValueError(f"the 8-bit KV cache takes head dims 64 and 128, got {head_dim}")
+            self.kv = KV8Layers(num_layers, num_pages, num_kv_heads, head_dim, self.device)
         self._alloc = _rt.PageAllocator(num_pages, 1) if _rt is not None else _PyAllocator(num_pages, 1)
         self.prefix_cache = None
 
@@ -73,12 +93,13 @@ class KVPool:
 
     @classmethod
     def for_memory(cls, num_layers, num_kv_heads, head_dim, bytes_budget: int, device, dtype=torch.bfloat16,
-                   max_pages: int | None = None):
-        per_page = num_layers * 2 * num_kv_heads * PAGE * head_dim * torch.finfo(dtype).bits // 8
+                   max_pages: int | None = None, kv_format: str = "native"):
+        row = head_dim * torch.finfo(dtype).bits // 8 if check_kv_format(kv_format) == "native" else head_dim + 1
+        per_page = num_layers * 2 * num_kv_heads * PAGE * row
         pages = max(2, int(bytes_budget // per_page))
         if max_pages is not None:
             pages = min(pages, max_pages)
-        return cls(num_layers, num_kv_heads, head_dim, pages, device, dtype)
+        return cls(num_layers, num_kv_heads, head_dim, pages, device, dtype, kv_format)
 
     def allocator_native(self):
         return self._alloc

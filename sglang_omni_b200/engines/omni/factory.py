@@ -34,11 +34,13 @@ def create_ar_engine(model, tokenizer=None, max_seq_len: int | None = None, devi
     """AR engine over the paged engine.  ``model``: a ``DecoderLM``, or a transformers causal LM
     (Llama / Mistral / Qwen2 / Qwen3 / Qwen3-MoE), converted first (``models.hf_text``), as the
     reference's factory takes any HF model; ``max_seq_len`` bounds a request's context;
+    ``kv_format="e4m3"`` keeps the KV cache in 8 bits (needed for sliding-window models);
     ``tokenizer`` is accepted for the reference's signature (detokenising happens in the stage)."""
     from ...models.decoder import DecoderLM
     from ..ar import AREngine, KVPool
     from ..ar.adapter import PagedAREngineAdapter
 
+    kv_format = kw.pop("kv_format", "native")
     if max_seq_len is not None:
         kw.setdefault("max_context", int(max_seq_len))
     if not isinstance(model, DecoderLM):
@@ -47,8 +49,8 @@ def create_ar_engine(model, tokenizer=None, max_seq_len: int | None = None, devi
         from ...models.hf_text.convert import eos_token_ids
 
         kw.setdefault("eos_token_ids", eos_token_ids(model))
-        model = decoder_from_hf(model, device or "cpu", max_position=kw.get("max_context"))
+        model = decoder_from_hf(model, device or "cpu", max_position=kw.get("max_context"), kv_format=kv_format)
     cfg = model.cfg
     pages = kw.pop("kv_pages", None) or (kw.get("max_batch", 64) * ((kw.get("max_context", 4096) + 63) // 64) + 8)
-    pool = KVPool(cfg.num_layers, cfg.num_kv_heads, cfg.head_dim, pages, model.embed.device, cfg.dtype)
+    pool = KVPool(cfg.num_layers, cfg.num_kv_heads, cfg.head_dim, pages, model.embed.device, cfg.dtype, kv_format)
     return PagedAREngineAdapter(AREngine(model, pool, **kw))

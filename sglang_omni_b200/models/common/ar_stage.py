@@ -41,8 +41,9 @@ def prompt_ids_of(data: Any) -> list[int]:
 def create_ar_executor(model, stage_name: str, tokenizer, max_batch: int = 64, max_context: int = 4096,
                        max_prefill_tokens: int = 8192, kv_pages: int | None = None, use_graphs: bool = True,
                        eos_token_ids=(), default_max_new_tokens: int = 128, prefix_cache: bool = True,
-                       rank_group=None) -> EngineExecutor:
-    """``rank_group``: a ``parallel.rank_group.GroupSpec`` (builder, mode, world, GPUs); the stage is
+                       rank_group=None, kv_format: str = "native") -> EngineExecutor:
+    """``kv_format``: ``native`` or ``e4m3`` (the 8-bit KV pool).
+    ``rank_group``: a ``parallel.rank_group.GroupSpec`` (builder, mode, world, GPUs); the stage is
     then served by that group (this process is its leader) and ``model`` is ignored."""
     dev = model.embed.device if model is not None else (torch.device("cuda", torch.cuda.current_device())
                                                         if rank_group is not None and rank_group.gpus
@@ -56,12 +57,13 @@ def create_ar_executor(model, stage_name: str, tokenizer, max_batch: int = 64, m
 
         rank_group.engine_args = engine_args
         rank_group.kv_pages = pages
+        rank_group.kv_format = kv_format
         rg = StageRankGroup(rank_group)
         engine = rg.start()
         adapter = PagedAREngineAdapter(engine, threaded=GroupedAREngine(engine, rg))
     else:
         cfg = model.cfg
-        pool = KVPool(cfg.num_layers, cfg.num_kv_heads, cfg.head_dim, pages, dev, cfg.dtype)
+        pool = KVPool(cfg.num_layers, cfg.num_kv_heads, cfg.head_dim, pages, dev, cfg.dtype, kv_format)
         engine = AREngine(model, pool, **engine_args)
         adapter = PagedAREngineAdapter(engine)
     detoks: dict[str, IncrementalDetokenizer] = {}

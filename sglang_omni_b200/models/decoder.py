@@ -66,11 +66,20 @@ class DecoderConfig:
     attention_bias: bool = False        # q / k / v projection biases (Qwen2)
     tie_word_embeddings: bool = False
     max_position: int = 65536
+    sliding_window: int = 0             # > 0: attention sees its last `sliding_window` keys (8-bit KV pools only)
+    window_layers: tuple | None = None  # layers with the window (None: all)
+    sink_tokens: int = 0                # first tokens that windowed layers keep seeing
     dtype: torch.dtype = torch.bfloat16
     name: str = "decoder"
 
     def is_moe_layer(self, i: int) -> bool:
         return self.num_experts > 0 and i >= self.first_k_dense and i not in self.mlp_only_layers
+
+    def window_of(self, i: int) -> tuple[int, int]:
+        """(window, sinks) of layer i; (0, 0) sees the whole context."""
+        if self.sliding_window <= 0 or (self.window_layers is not None and i not in self.window_layers):
+            return 0, 0
+        return self.sliding_window, self.sink_tokens
 
     @property
     def q_size(self):
@@ -378,8 +387,6 @@ class DecoderLM(nn.Module):
             return self._forward_tp(fb, kv_cache, res)
         h = None
         fused_next = None    # this layer's input norm, already done by the previous MoE combine
-        rot = cfg.rotary_dim or cfg.head_dim
-        scale = 1.0 / math.sqrt(cfg.head_dim)
         nl = len(self.layers)
         for i, L in enumerate(self.layers):
             if fused_next is not None:
@@ -391,17 +398,7 @@ class DecoderLM(nn.Module):
             if i in fb.capture_layers:
                 fb.captured[i] = res.clone()
             qkv = ops.linear(normed, L.qkv, bias=getattr(L, "qkv_bias", None))
-            ops.qkv_rope_store(qkv, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, fb.positions, self.cos_tab,
-                               self.sin_tab, rot, getattr(L, "q_norm", None), getattr(L, "k_norm", None),
-                               cfg.rms_norm_eps, cfg.rope_neox, cfg.mrope_section, cfg.mrope_interleaved,
-                               fb.slot_mapping, kv_cache[i, 0], kv_cache[i, 1])
-            if fb.is_decode:
-                attn = ops.decode_attention(qkv, kv_cache[i, 0], kv_cache[i, 1], fb.block_table, fb.kv_lens,
-                                            cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, self._dec_ws, scale)
-            else:
-                attn = ops.prefill_attention(qkv, kv_cache[i, 0], kv_cache[i, 1], fb.block_table, fb.cu_q,
-                                             fb.kv_lens, fb.tile_req, fb.tile_tok0, cfg.num_heads,
-                                             cfg.num_kv_heads, cfg.head_dim, scale, tile_rows=fb.tile_rows)
+            attn = self._attend(L, i, qkv, fb, kv_cache)
             o = ops.linear(attn, L.o)
             normed2 = ops.rms_norm(o, L.ln2, cfg.rms_norm_eps, residual=res)
             has_ds = fb.deepstack is not None and i < len(fb.deepstack) and fb.deepstack[i] is not None
@@ -420,8 +417,26 @@ class DecoderLM(nn.Module):
         return ops.rms_norm(h, self.final_norm, cfg.rms_norm_eps, residual=res)
 
     def _attention(self, L, i, normed, fb, kv_cache, wait=None):
+        return self._attend(L, i, ops.linear(normed, L.qkv, bias=getattr(L, "qkv_bias", None), wait=wait), fb, kv_cache)
+
+    def _attend(self, L, i, qkv, fb, kv_cache):
+        """Norm + RoPE + cache write of layer i's QKV rows, and their attention over the cache
+        (in the model's dtype, or ``ops.KV8Layers``)."""
         cfg = self.cfg
-        qkv = ops.linear(normed, L.qkv, bias=getattr(L, "qkv_bias", None), wait=wait)
+        window, sinks = cfg.window_of(i)
+        if isinstance(kv_cache, ops.KV8Layers):
+            cache = kv_cache[i]
+            q = ops.kv8_store(qkv, cache, fb.slot_mapping, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, fb.positions,
+                              self.cos_tab, self.sin_tab, cfg.rotary_dim or cfg.head_dim, getattr(L, "q_norm", None),
+                              getattr(L, "k_norm", None), cfg.rms_norm_eps, cfg.rope_neox, cfg.mrope_section,
+                              cfg.mrope_interleaved)
+            if fb.is_decode:
+                return ops.kv8_decode_attention(q, cache, fb.block_table, fb.kv_lens, cfg.num_heads, cfg.num_kv_heads,
+                                                cfg.head_dim, window=window, sinks=sinks)
+            return ops.kv8_prefill_attention(q, cache, fb.block_table, fb.cu_q, fb.kv_lens, cfg.num_heads,
+                                             cfg.num_kv_heads, cfg.head_dim, window=window, sinks=sinks)
+        if window > 0:
+            raise ValueError(f"layer {i} has a sliding window of {window}: serve it with an 8-bit KV pool (kv_format='e4m3')")
         ops.qkv_rope_store(qkv, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, fb.positions, self.cos_tab,
                            self.sin_tab, cfg.rotary_dim or cfg.head_dim, getattr(L, "q_norm", None),
                            getattr(L, "k_norm", None), cfg.rms_norm_eps, cfg.rope_neox, cfg.mrope_section,

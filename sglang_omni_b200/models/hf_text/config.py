@@ -17,7 +17,8 @@ _P = "sglang_omni_b200.models"
 
 
 def hf_text_stages(device: str = "cuda:0", max_batch: int = 64, max_context: int = 4096,
-                   max_prefill_tokens: int = 8192, use_graphs: bool = True) -> list[StageConfig]:
+                   max_prefill_tokens: int = 8192, use_graphs: bool = True,
+                   kv_format: str = "native") -> list[StageConfig]:
     return [
         StageConfig(name="preprocessing",
                     executor=ExecutorConfig(factory=f"{_P}.hf_text.config.create_hf_preprocessing_executor"),
@@ -27,7 +28,7 @@ def hf_text_stages(device: str = "cuda:0", max_batch: int = 64, max_context: int
                                             args={"device": device, "max_batch": max_batch,
                                                   "max_context": max_context,
                                                   "max_prefill_tokens": max_prefill_tokens,
-                                                  "use_graphs": use_graphs}),
+                                                  "use_graphs": use_graphs, "kv_format": kv_format}),
                     get_next=f"{_P}.common.text_stages.terminal"),
     ]
 
@@ -59,7 +60,9 @@ def create_hf_preprocessing_executor(model_path: str = ""):
 
 def create_hf_decoder_executor(model_path: str = "", device: str = "cuda:0", max_batch: int = 64,
                                max_context: int = 4096, max_prefill_tokens: int = 8192, use_graphs: bool = True,
-                               dtype: str | None = None, default_max_new_tokens: int = 256):
+                               dtype: str | None = None, default_max_new_tokens: int = 256,
+                               kv_format: str = "native"):
+    """``kv_format="e4m3"``: the 8-bit KV pool, which sliding-window checkpoints need."""
     import torch
 
     from ..common.ar_stage import create_ar_executor
@@ -68,11 +71,12 @@ def create_hf_decoder_executor(model_path: str = "", device: str = "cuda:0", max
 
     dt = {"bf16": torch.bfloat16, "bfloat16": torch.bfloat16, "fp16": torch.float16, "float16": torch.float16,
           "fp32": torch.float32, "float32": torch.float32}.get(dtype) if dtype else None
-    model = decoder_from_hf(model_path, device, dt, max_position=max_context)
+    model = decoder_from_hf(model_path, device, dt, max_position=max_context, kv_format=kv_format)
     tok = load_tokenizer(model_path, model.cfg.vocab_size)
     return create_ar_executor(model, "decoder", tok, max_batch=max_batch, max_context=max_context,
                               max_prefill_tokens=max_prefill_tokens, use_graphs=use_graphs,
-                              eos_token_ids=eos_token_ids(model_path), default_max_new_tokens=default_max_new_tokens)
+                              eos_token_ids=eos_token_ids(model_path), default_max_new_tokens=default_max_new_tokens,
+                              kv_format=kv_format)
 
 
 EntryClass = HFTextPipelineConfig

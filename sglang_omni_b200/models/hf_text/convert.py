@@ -10,9 +10,10 @@ tcgen05 GEMM / attention kernels like the omni models do.
 Covered configuration fields: GQA heads and head_dim, q / k / v biases (Qwen2; Llama's
 ``attention_bias``), per-head q / k RMSNorm (Qwen3), RoPE theta with linear or Llama-3 frequency
 scaling, tied embeddings, softmax top-k routed experts with optional top-k renormalisation and
-dense ``mlp_only_layers`` / ``decoder_sparse_step`` layers (Qwen3-MoE).  Refused with a message:
-sliding-window attention (Mistral v0.1 style, Qwen2 ``use_sliding_window``), MLP biases, other
-RoPE scalings."""
+dense ``mlp_only_layers`` / ``decoder_sparse_step`` layers (Qwen3-MoE); with the 8-bit KV pool
+(``kv_format="e4m3"``) sliding-window attention (Mistral v0.1 style, Qwen2 ``use_sliding_window``
+from ``max_window_layers`` on, ``layer_types``).  Refused with a message: sliding windows with the
+native KV pool, MLP biases, other RoPE scalings."""
 from __future__ import annotations
 
 import json
@@ -41,7 +42,8 @@ def _rope(c) -> tuple[float, dict | None]:
     return float(theta), (dict(scaling) if scaling else None)
 
 
-def decoder_config_from_hf(c: Any, dtype: torch.dtype = torch.bfloat16, max_position: int | None = None) -> DecoderConfig:
+def decoder_config_from_hf(c: Any, dtype: torch.dtype = torch.bfloat16, max_position: int | None = None,
+                           kv_format: str = "native") -> DecoderConfig:
     """``c``: a transformers ``PretrainedConfig`` or its ``config.json`` dict."""
     archs = list(_get(c, "architectures") or [])
     arch = archs[0] if archs else ""
@@ -53,7 +55,15 @@ def decoder_config_from_hf(c: Any, dtype: torch.dtype = torch.bfloat16, max_posi
     win = _get(c, "sliding_window")
     if win and (_get(c, "use_sliding_window", arch != "Qwen2ForCausalLM") and int(win) < int(
             max_position or _get(c, "max_position_embeddings") or 0)):
-        raise NotImplementedError(f"{arch}: sliding-window attention ({win}) is not supported by the paged engine")
+        if kv_format == "native":
+            raise NotImplementedError(f"{arch}: sliding-window attention ({win}) is not supported by the paged engine's "
+                                      "native KV pool; kv_format='e4m3' serves it")
+        kinds = list(_get(c, "layer_types") or [])
+        first = int(_get(c, "max_window_layers") or 0) if arch.startswith("Qwen") else 0
+        window = dict(sliding_window=int(win), window_layers=tuple(
+            i for i in range(layers) if (kinds[i] == "sliding_attention" if len(kinds) == layers else i >= first)))
+    else:
+        window = {}
     if _get(c, "mlp_bias", False):
         raise NotImplementedError(f"{arch}: MLP biases are not supported")
     theta, scaling = _rope(c)
@@ -70,7 +80,7 @@ def decoder_config_from_hf(c: Any, dtype: torch.dtype = torch.bfloat16, max_posi
               rope_neox=True, qk_norm=qwen3, attention_bias=bool(qwen2 or _get(c, "attention_bias", False)),
               tie_word_embeddings=bool(_get(c, "tie_word_embeddings", False)),
               max_position=int(max_position or _get(c, "max_position_embeddings") or 32768), dtype=dtype,
-              name=(arch or "hf_causal_lm").lower())
+              name=(arch or "hf_causal_lm").lower(), **window)
     experts = int(_get(c, "num_experts") or 0)
     if experts:
         step = int(_get(c, "decoder_sparse_step") or 1)
@@ -107,10 +117,11 @@ def eos_token_ids(src: Any) -> tuple[int, ...]:
 
 @torch.no_grad()
 def decoder_from_hf(src: Any, device="cpu", dtype: torch.dtype | None = None,
-                    max_position: int | None = None) -> DecoderLM:
+                    max_position: int | None = None, kv_format: str = "native") -> DecoderLM:
     """``src``: a transformers causal-LM module (its config and state dict are read) or a local
     checkpoint directory (config.json + safetensors).  ``dtype`` defaults to bf16 on a GPU and to
-    the checkpoint's dtype (fp32 for a module) on the CPU."""
+    the checkpoint's dtype (fp32 for a module) on the CPU; ``kv_format``: the KV pool it will be
+    served with."""
     dev = torch.device(device)
     if isinstance(src, str):
         with open(os.path.join(src, "config.json")) as f:
@@ -124,7 +135,7 @@ def decoder_from_hf(src: Any, device="cpu", dtype: torch.dtype | None = None,
         ck = next(src.parameters()).dtype
     if dtype is None:
         dtype = torch.bfloat16 if dev.type == "cuda" else ck
-    cfg = decoder_config_from_hf(c, dtype, max_position)
+    cfg = decoder_config_from_hf(c, dtype, max_position, kv_format)
     model = DecoderLM(cfg, device=dev)
     load_decoder_from_hf(model, sd, "model.", "lm_head.weight")
     return model

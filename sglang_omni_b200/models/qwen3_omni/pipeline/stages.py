@@ -270,14 +270,17 @@ def create_thinker_executor(model_path: str = "", device: str = "cuda:0", max_ba
                             max_context: int = 4096, max_prefill_tokens: int = 8192, speech_target: str | None = None,
                             accept_hidden_layer: int = 24, overrides: dict | None = None, use_graphs: bool = True,
                             model=None, tokenizer=None, eos_token_ids=THINKER_EOS_IDS, prefix_cache: bool = True,
-                            tp_size: int = 1, ep_size: int = 1, gpus: list | None = None):
+                            tp_size: int = 1, ep_size: int = 1, gpus: list | None = None,
+                            kv_format: str = "native"):
     """The thinker stage over the paged engine; ``model`` / ``tokenizer`` / ``eos_token_ids``
     let another omni model (same request layout: prompt ids + audio / image spans) reuse it.
 
     ``tp_size`` / ``ep_size`` > 1 serve the thinker with a rank group of that many GPUs
     (``gpus``: logical GPU per rank, default this device and the next ones): tensor
     parallel (every rank runs every request) or expert parallel with data-parallel
-    attention (each request on one rank, the experts sharded)."""
+    attention (each request on one rank, the experts sharded).
+
+    ``kv_format="e4m3"`` keeps the KV cache in 8 bits: about half the bytes per token."""
     dev = torch.device(device)
     pages = max_batch * ((max_context + 63) // 64) + 8
     engine_args = dict(max_batch=max_batch, max_prefill_tokens=max_prefill_tokens, max_context=max_context,
@@ -304,7 +307,7 @@ def create_thinker_executor(model_path: str = "", device: str = "cuda:0", max_ba
                          builder="sglang_omni_b200.models.qwen3_omni.loader.build_thinker_rank",
                          builder_args={"model_path": model_path, "overrides": overrides,
                                        "max_tokens": max(max_prefill_tokens, max_batch)},
-                         engine_args=engine_args, kv_pages=pages, tp=group_tp)
+                         engine_args=engine_args, kv_pages=pages, tp=group_tp, kv_format=kv_format)
         rg = StageRankGroup(spec)
         engine = rg.start()
         model = rg.model
@@ -312,7 +315,7 @@ def create_thinker_executor(model_path: str = "", device: str = "cuda:0", max_ba
     else:
         model = model if model is not None else loader.get_thinker(model_path, dev, overrides)
         cfg = model.cfg
-        pool = KVPool(cfg.num_layers, cfg.num_kv_heads, cfg.head_dim, pages, dev, cfg.dtype)
+        pool = KVPool(cfg.num_layers, cfg.num_kv_heads, cfg.head_dim, pages, dev, cfg.dtype, kv_format)
         engine = AREngine(model, pool, **engine_args)
         adapter = PagedAREngineAdapter(engine)
     tok = tokenizer if tokenizer is not None else load_tokenizer(model_path, model.cfg.vocab_size)

@@ -46,6 +46,22 @@ class KV8Cache:
         return cls(codes[0], codes[1], exps[0], exps[1])
 
 
+class KV8Layers:
+    """The 8-bit caches of all layers of a pool; ``[i]`` is layer i's :class:`KV8Cache`."""
+
+    def __init__(self, num_layers: int, num_pages: int, num_kv_heads: int, head_dim: int, device):
+        codes = torch.zeros(num_layers, 2, num_pages, num_kv_heads, PAGE, head_dim, dtype=torch.uint8, device=device)
+        self.codes = codes.view(torch.float8_e4m3fn)
+        self.exps = torch.zeros(num_layers, 2, num_pages, num_kv_heads, PAGE, dtype=torch.int8, device=device)
+        self.layers = [KV8Cache(c[0], c[1], e[0], e[1]) for c, e in zip(self.codes, self.exps)]
+
+    def __len__(self) -> int:
+        return len(self.layers)
+
+    def __getitem__(self, i: int) -> KV8Cache:
+        return self.layers[i]
+
+
 # ---------------------------------------------------------------- plain restatements (CPU path, test oracles)
 def kv8_quantize_ref(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows x [..., D] -> (codes float8_e4m3fn, exponents int8)."""

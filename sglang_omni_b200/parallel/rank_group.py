@@ -73,6 +73,7 @@ class GroupSpec:
     builder_args: dict = field(default_factory=dict)
     engine_args: dict = field(default_factory=dict)
     kv_pages: int = 0
+    kv_format: str = "native"                   # KVPool format of every rank
     host: str = "127.0.0.1"
     store_port: int = 0
     pub_port: int = 0
@@ -113,7 +114,8 @@ def _build_rank(spec: GroupSpec, rank: int, device: torch.device):
     args.setdefault("tp", spec.tp)
     model = import_string(spec.builder)(args, rank, spec.world, device, group, spec.mode)
     cfg = model.cfg
-    pool = KVPool(cfg.num_layers, cfg.num_kv_heads, cfg.head_dim, spec.kv_pages, device, cfg.dtype)
+    pool = KVPool(cfg.num_layers, cfg.num_kv_heads, cfg.head_dim, spec.kv_pages, device, cfg.dtype,
+                  spec.kv_format)
     eng = AREngine(model, pool, **spec.engine_args)
     return group, model, eng
 
