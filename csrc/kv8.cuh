@@ -25,8 +25,8 @@ constexpr int kExpMin = -60;
 constexpr int kExpMax = 60;
 constexpr int kExpBad = -128;
 
-// 2^e of a row's exponent byte; NaN for a row that is not finite.  Exponents outside the format's
-// range (a cache that was never written) are clamped into it.
+// 2^e of a row's exponent byte; NaN for a row that is not finite.  Other exponents outside the format's
+// range are clamped into it (a cache that was never written).
 __device__ __forceinline__ float pow2_of(int e) {
   if (e == kExpBad) return __int_as_float(0x7fc00000);
   e = max(kExpMin, min(kExpMax, e));

@@ -13,8 +13,8 @@
 //   does not depend on them (CUDA graphs).  A pair that lies in several CTAs leaves partial sums,
 //   which a second, dependent launch joins in a fixed order.
 // * A producer warp issues TMA loads (K and V tile swizzled, their exponents as bulk copies);
-//   four consumer warps take 16 keys of every tile each and keep their own running maximum, sum
-//   and output until the pair ends, so tiles need no barrier among the warps.
+//   two pairs of consumer warps take the tiles in turn, each warp 32 of the 64 keys, and keep their own
+//   running maximum, sum and output until the pair ends, so tiles need no barrier among the warps.
 // * Arithmetic on 16 keys: the codes go to fp16 (exact), S^T = K Q^T and O^T += V^T P by
 //   mma.m16n8k16 with the keys / dims as the 16 rows and the query heads of the KV head as the
 //   columns, so few heads waste few rows.  The contraction order inside a 16-dim chunk is free, and
@@ -31,6 +31,7 @@
 #include <cuda_runtime.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "host_util.h"
 #include "kv8.cuh"
@@ -50,14 +51,11 @@ constexpr float kHead = 7.f;                    // weights are held times 2^7: b
 
 template <int D, int NT>
 struct Smem {
-#ifndef ST128
-#define ST128 3
-#define ST64 5
-#define CT128 3
-#define CT64 4
-#endif
-  static constexpr int kCtas = D == 128 ? (NT == 1 ? CT128 : 2) : (NT == 1 ? CT64 : 3);   // resident per SM
-  static constexpr int kStages = D == 128 ? (NT == 1 ? ST128 : 4) : ST64;
+  // CTAs per SM and ring depth: 64 slots of about 1150 keys, 5 of 52,000 - 130,000 and 48 windows of 4096
+  // (head dim 64) took, in microseconds, at (CTAs, stages) (2, 5): 26.3, 212, 62; (3, 3 | 64: 5): 26.3, 208, 56;
+  // (3, 3 | 64: 4 CTAs, 5 stages): 26.1, 207, 53.
+  static constexpr int kCtas = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
+  static constexpr int kStages = D == 128 ? (NT == 1 ? 3 : 4) : 5;
   static constexpr int kTile = kPage * D;       // bytes of a K or V tile
   static constexpr int kStage = 2 * kTile;
   static constexpr int kExp = kStages * kStage;                 // exponents: [stage][2][64]
@@ -307,8 +305,10 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
 
   // -------------------------------------------------------------- consumers
   const int g = lane >> 2, t4 = lane & 3;
-  const int lrow = warp * 16 + (lane & 15);                 // ldmatrix row of this lane
-  int s = 0;                      // ring stage and phase
+  const int row0 = (warp & 1) * 32;                         // keys of the tile that this warp takes
+  const int lrow = row0 + (lane & 15);                      // ldmatrix row of this lane
+  uint32_t t0 = 0;                // tiles before this one
+  int s = 0;                      // their ring stage and phase
   uint32_t ph = 0;
   bool ok = true;
   bool more = true;
@@ -359,63 +359,63 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
       l[nt][0] = l[nt][1] = 0.f;
     }
 
-    for (int i = w.i0; i < w.i1; ++i) {
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], ph, abort_flag, p.status));
-      if (!ok) continue;
-      const uint32_t kt = smem_u32(smem + s * S::kStage), vt = kt + S::kTile;
-      const int8_t* ex = reinterpret_cast<const int8_t*>(smem + S::kExp + s * 2 * kPage) + warp * 16;
-      const int key0 = sp.tile(i) * kPage;
-      const bool edge = key0 + kPage > sp.kv || (key0 < sp.lo && key0 + kPage > sp.sinks);
-
-      // S^T: 16 keys x 8 NT heads
-      float sc[NT][4];
+    // 32 keys of the tile in ring stage s, two groups of 16.  kEdge: some of its keys are not visible.
+    auto work = [&](int stage, int key0, auto edge_tag) {
+      constexpr bool kEdge = decltype(edge_tag)::value;
+      const uint32_t kt = smem_u32(smem + stage * S::kStage), vt = kt + S::kTile;
+      const int8_t* ex = reinterpret_cast<const int8_t*>(smem + S::kExp + stage * 2 * kPage) + row0 + g;
+      auto seen = [&](int key) { return key < sp.kv && (key >= sp.lo || key < sp.sinks); };
+      // S^T: 2 x 16 keys x 8 NT heads
+      float x[2][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+      for (int q = 0; q < 2; ++q)
 #pragma unroll
-      for (int c = 0; c < C; c += 2) {
-        uint32_t r[4];
-        ldsm4(kt + swz<D>(lrow, c + (lane >> 4)), r);
+        for (int nt = 0; nt < NT; ++nt) x[q][nt][0] = x[q][nt][1] = x[q][nt][2] = x[q][nt][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; c += 2)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t r[4];
+          ldsm4(kt + swz<D>(lrow + 16 * q, c + (lane >> 4)), r);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_to_f16x4(r[2 * u], a0, a2);
+            e4m3x4_to_f16x4(r[2 * u + 1], a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma(x[q][nt], a0, a1, a2, a3, qf[nt][c + u][0], qf[nt][c + u][1]);
+          }
+        }
+      // log2 weights on the codes: score + V's exponent; NaN where either row is marked as not finite
+      float vi[2][2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          uint32_t a0, a1, a2, a3;
-          e4m3x4_to_f16x4(r[2 * u], a0, a2);
-          e4m3x4_to_f16x4(r[2 * u + 1], a1, a3);
+          const int ke = ex[16 * q + 8 * u], ve = ex[kPage + 16 * q + 8 * u];
+          const float kf = __int_as_float(0x3f800000 + (ke << 23));
+          const float vf = min(ke, ve) == kExpBad ? __int_as_float(0x7fc00000) : __int_as_float(0x4b400000 + ve) - 12582912.f;
+          vi[q][u] = __int_as_float(0x3f800000 - (ve << 23));
+          const bool in = !kEdge || seen(key0 + row0 + 16 * q + 8 * u + g);
+          if (!in) vi[q][u] = 0.f;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma(sc[nt], a0, a1, a2, a3, qf[nt][c + u][0], qf[nt][c + u][1]);
-        }
-      }
-      // weights
-      float kf[2], ve[2], vi[2];
-      bool vis[2] = {true, true};
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int j = g + 8 * u;
-        const int ev = ex[kPage + j];
-        const int ec = max(kExpMin, min(kExpMax, ev));
-        kf[u] = pow2_of(ex[j]);
-        ve[u] = ev == kExpBad ? __int_as_float(0x7fc00000) : static_cast<float>(ec);
-        vi[u] = __int_as_float((127 - ec) << 23);
-        if (edge) {
-          const int key = key0 + warp * 16 + j;
-          vis[u] = key < sp.kv && (key >= sp.lo || key < sp.sinks);
+            for (int v = 0; v < 2; ++v) {
+              x[q][nt][2 * u + v] = fmaf(x[q][nt][2 * u + v], qs[nt][v] * kf, vf);
+              if (!in) x[q][nt][2 * u + v] = -INFINITY;
+            }
         }
-      }
-      uint32_t pb[NT][2];
+      uint32_t pb[2][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float x[4];
+        float top[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            x[2 * u + v] = fmaf(sc[nt][2 * u + v], qs[nt][v] * kf[u], ve[u]);
-            if (!vis[u]) x[2 * u + v] = -INFINITY;
-          }
-        const bool grow = x[0] > m[nt][0] + kRaise || x[2] > m[nt][0] + kRaise || x[1] > m[nt][1] + kRaise || x[3] > m[nt][1] + kRaise;
-        if (__any_sync(0xffffffffu, grow)) {
+        for (int v = 0; v < 2; ++v) top[v] = fmaxf(fmaxf(x[0][nt][v], x[0][nt][2 + v]), fmaxf(x[1][nt][v], x[1][nt][2 + v]));
+        if (__any_sync(0xffffffffu, top[0] > m[nt][0] + kRaise || top[1] > m[nt][1] + kRaise)) {
 #pragma unroll
           for (int v = 0; v < 2; ++v) {
-            float mx = fmaxf(x[v], x[2 + v]);
+            float mx = top[v];
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -430,40 +430,65 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
             }
           }
         }
+        float less[2];
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const float sub = m[nt][v] == -INFINITY ? 0.f : m[nt][v] - kHead;
-          x[v] = ex2(x[v] - sub);
-          x[2 + v] = ex2(x[2 + v] - sub);
-          l[nt][v] += x[v] * vi[0] + x[2 + v] * vi[1];
-        }
-        pb[nt][0] = movm_t(pack_h2(x[0], x[1]));
-        pb[nt][1] = movm_t(pack_h2(x[2], x[3]));
-      }
-      // O^T += V^T P; keys outside the visible range may hold anything: their codes become zeros
-      uint32_t keep[2] = {~0u, ~0u};
-      if (edge) {
+        for (int v = 0; v < 2; ++v) less[v] = m[nt][v] == -INFINITY ? 0.f : kHead - m[nt][v];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int key = key0 + warp * 16 + 8 * u + 2 * t4;
-          const bool a = key < sp.kv && (key >= sp.lo || key < sp.sinks);
-          const bool b = key + 1 < sp.kv && (key + 1 >= sp.lo || key + 1 < sp.sinks);
-          keep[u] = (a ? 0xffffu : 0u) | (b ? 0xffff0000u : 0u);
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            x[q][nt][v] = ex2(x[q][nt][v] + less[v]);
+            x[q][nt][2 + v] = ex2(x[q][nt][2 + v] + less[v]);
+            l[nt][v] = fmaf(x[q][nt][v], vi[q][0], fmaf(x[q][nt][2 + v], vi[q][1], l[nt][v]));
+          }
+          pb[q][nt][0] = movm_t(pack_h2(x[q][nt][0], x[q][nt][1]));
+          pb[q][nt][1] = movm_t(pack_h2(x[q][nt][2], x[q][nt][3]));
         }
       }
+      // O^T += V^T P; keys that are not visible may hold anything: their codes become zeros
+      uint32_t keep[2][2];
+      if constexpr (kEdge) {
 #pragma unroll
-      for (int c = 0; c < C; c += 2) {
-        uint32_t r[4];
-        ldsm4_t(vt + swz<D>(lrow, c + (lane >> 4)), r);
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          // bytes (key 2t: dims 2g, 2g+1; key 2t+1: the same) -> two keys of a dim side by side
-          uint32_t a0, a1, a2, a3;
-          e4m3x4_to_f16x4(__byte_perm(r[2 * u] & keep[0], 0u, 0x3120), a0, a1);
-          e4m3x4_to_f16x4(__byte_perm(r[2 * u + 1] & keep[1], 0u, 0x3120), a2, a3);
+          for (int u = 0; u < 2; ++u) {
+            const int key = key0 + row0 + 16 * q + 8 * u + 2 * t4;
+            keep[q][u] = (seen(key) ? 0xffffu : 0u) | (seen(key + 1) ? 0xffff0000u : 0u);
+          }
+      }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma(o[nt][c + u], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+      for (int c = 0; c < C; c += 2)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t r[4];
+          ldsm4_t(vt + swz<D>(lrow + 16 * q, c + (lane >> 4)), r);
+          if constexpr (kEdge) {
+            r[0] &= keep[q][0], r[2] &= keep[q][0];
+            r[1] &= keep[q][1], r[3] &= keep[q][1];
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            // bytes (key 2t: dims 2g, 2g+1; key 2t+1: the same) -> two keys of a dim side by side
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_to_f16x4(__byte_perm(r[2 * u], 0u, 0x3120), a0, a1);
+            e4m3x4_to_f16x4(__byte_perm(r[2 * u + 1], 0u, 0x3120), a2, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma(o[nt][c + u], a0, a1, a2, a3, pb[q][nt][0], pb[q][nt][1]);
+          }
         }
+    };
+
+    // The two pairs of warps take tiles in turn.  Every warp waits for every tile and releases it, so that
+    // no stage is filled again before all have seen it: a phase's parity tells only the last two apart.
+    for (int i = w.i0; i < w.i1; ++i, ++t0) {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], ph, abort_flag, p.status));
+      if (!ok) break;
+      if ((t0 & 1) == static_cast<uint32_t>(warp >> 1)) {
+        const int key0 = sp.tile(i) * kPage;
+        if (key0 + kPage > sp.kv || (key0 < sp.lo && key0 + kPage > sp.sinks))
+          work(s, key0, std::true_type{});
+        else
+          work(s, key0, std::false_type{});
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
