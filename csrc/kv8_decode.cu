@@ -11,7 +11,8 @@
 //   the tiles [c * per, (c + 1) * per) of it, per = ceil(tiles / CTAs), found on the device from
 //   kv_lens.  Every CTA streams the same number of tiles whatever the lengths are, and the launch
 //   does not depend on them (CUDA graphs).  A pair that lies in several CTAs leaves partial sums,
-//   which a second, dependent launch joins in a fixed order.
+//   which a second, dependent launch joins in a fixed order.  Where the pairs alone occupy the GPU
+//   evenly, each CTA takes one whole pair.
 // * A producer warp issues TMA loads (K and V tile swizzled, their exponents as bulk copies);
 //   two pairs of consumer warps take the tiles in turn, each warp 32 of the 64 keys, and keep their own
 //   running maximum, sum and output until the pair ends, so tiles need no barrier among the warps.
@@ -122,18 +123,36 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
   return v;
 }
 
-// Tiles of all requests, and of those before request `stop` (whole warp).
-__device__ __forceinline__ int64_t count_tiles(const Params& p, int stop, int64_t* before) {
-  const int lane = threadIdx.x & 31;
-  int64_t all = 0, head = 0;
-  for (int b = lane; b < p.batch; b += 32) {
-    const int n = Span(p, b).tiles;
-    all += n;
-    if (b < stop) head += n;
+// How the tiles are dealt out (whole warp; the same in every warp of both launches).
+struct Plan {
+  int64_t tiles;          // of one (KV head, head group), over all requests
+  int64_t before;         // of them, in the requests before `stop`
+  int64_t per;            // tiles of a CTA
+  int64_t pairs;          // with a visible key
+  bool whole;             // a pair per CTA instead
+  __device__ Plan(const Params& p, int R, int stop) {
+    const int lane = threadIdx.x & 31;
+    int64_t all = 0, head = 0;
+    int live = 0, most = 0;
+    for (int b = lane; b < p.batch; b += 32) {
+      const int n = Span(p, b).tiles;
+      all += n;
+      if (b < stop) head += n;
+      live += n > 0;
+      most = max(most, n);
+    }
+    tiles = warp_sum64(all);
+    before = warp_sum64(head);
+    live = __reduce_add_sync(0xffffffffu, live);
+    most = __reduce_max_sync(0xffffffffu, most);
+    per = (tiles * R + p.ctas - 1) / p.ctas;
+    // Pairs of nearly equal lengths that occupy a good part of the CTAs keep the memory busy without
+    // being split, and save the second segment of each CTA and the joining: 64 slots of about 1150 keys
+    // 21.8 us split, WHOLE64 whole; 48 windows of 4096 (head dim 64) 47.7 and WHOLEW.
+    pairs = static_cast<int64_t>(live) * R;
+    whole = pairs <= p.ctas && 5 * pairs >= 2 * p.ctas && 4 * static_cast<int64_t>(most) * live <= 5 * tiles;
   }
-  if (before != nullptr) *before = warp_sum64(head);
-  return warp_sum64(all);
-}
+};
 
 // Walks a CTA's tiles pair by pair (whole warp; every warp of the CTA walks alike).
 struct Walk {
@@ -141,33 +160,41 @@ struct Walk {
   int i0, i1, n;          // this segment's tiles [i0, i1) of the pair's n
   int64_t left;
   int per_b;              // pairs per request
-  __device__ Walk(const Params& p, int64_t x0, int64_t x1, int R) {
+  // tiles [x, x + count) of all pairs', or pair x whole
+  __device__ Walk(const Params& p, const Plan& plan, int64_t x, int64_t count, int R) {
     per_b = R;
-    left = x1 - x0;
+    left = count;
     const int lane = threadIdx.x & 31;
     int64_t cum = 0;
     b = 0;
     for (int base = 0; base < p.batch; base += 32) {
       const int mine = base + lane < p.batch ? Span(p, base + lane).tiles : 0;
-      int64_t inc = mine;
+      const int64_t weight = plan.whole ? (mine > 0 ? 1 : 0) : mine;
+      int64_t inc = weight;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int64_t up = __shfl_up_sync(0xffffffffu, inc, d);
         if (lane >= d) inc += up;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, (cum + inc) * R > x0);
+      const unsigned past = __ballot_sync(0xffffffffu, (cum + inc) * R > x);
       if (past != 0) {
         const int at = __ffs(past) - 1;
         b = base + at;
         n = __shfl_sync(0xffffffffu, mine, at);
-        cum += __shfl_sync(0xffffffffu, inc - mine, at);
+        cum += __shfl_sync(0xffffffffu, inc - weight, at);
         break;
       }
       cum += __shfl_sync(0xffffffffu, inc, 31);
     }
-    const int64_t rel = x0 - cum * R;
-    r = static_cast<int>(rel / n);
-    i0 = static_cast<int>(rel - static_cast<int64_t>(r) * n);
+    const int64_t rel = x - cum * R;
+    if (plan.whole) {
+      r = static_cast<int>(rel);
+      i0 = 0;
+      left = n;
+    } else {
+      r = static_cast<int>(rel / n);
+      i0 = static_cast<int>(rel - static_cast<int64_t>(r) * n);
+    }
     i1 = static_cast<int>(min(static_cast<int64_t>(n), i0 + left));
   }
   __device__ bool next(const Params& p) {
@@ -251,15 +278,14 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
     tma_prefetch_desc(&tv);
   }
   __syncthreads();
-  grid_dep_launch();   // the joining launch may set up; it waits for this grid before it reads
   grid_dep_wait();
+  grid_dep_launch();   // after the wait: the joining launch may read kv_lens at once, and waits for the sums
 
   const int R = p.hkv * p.head_groups;
-  const int64_t W = count_tiles(p, 0, nullptr) * R;
-  const int64_t per = (W + p.ctas - 1) / p.ctas;
-  const int64_t x0 = blockIdx.x * per, x1 = min(W, x0 + per);
-  if (x0 >= x1) return;
-  Walk w(p, x0, x1, R);
+  const Plan plan(p, R, 0);
+  const int64_t x0 = plan.whole ? static_cast<int64_t>(blockIdx.x) : blockIdx.x * plan.per;
+  if (plan.whole ? x0 >= plan.pairs : x0 >= plan.tiles * R) return;
+  Walk w(p, plan, x0, min(plan.per, plan.tiles * R - x0), R);
 
   if (warp == kWarps) {
     // ------------------------------------------------------------ producer
@@ -555,24 +581,24 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
 template <int D, int NT, int W>
 __global__ void __launch_bounds__(128) kv8_decode_join_kernel(const Params p) {
   __shared__ float red[4 * D];
-  grid_dep_wait();   // in every thread: the grid before may itself still wait for what wrote kv_lens
+  // One thread's exit without the wait would let what follows on the stream start before the sums are
+  // written; the plan is read before it.
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / W) + (threadIdx.x >> 5) / W;
-  if (row >= static_cast<int64_t>(p.batch) * p.hq) return;
-  const int b = static_cast<int>(row / p.hq), hq = static_cast<int>(row - static_cast<int64_t>(b) * p.hq);
+  const bool live = row < static_cast<int64_t>(p.batch) * p.hq;
+  const int b = live ? static_cast<int>(row / p.hq) : 0, hq = live ? static_cast<int>(row - static_cast<int64_t>(b) * p.hq) : 0;
   const int h = hq / p.group, in = hq - h * p.group, hg = in / (8 * NT), head = in - hg * 8 * NT;
   const int R = p.hkv * p.head_groups;
-  int64_t before;
-  const int64_t all = count_tiles(p, b, &before) * R;
+  const Plan plan(p, R, b);
   const int n = Span(p, b).tiles;
   int64_t c0 = 0;
   int count = 0;
   if (n > 0) {
-    const int64_t per = (all + p.ctas - 1) / p.ctas;
-    const int64_t x = before * R + static_cast<int64_t>(h * p.head_groups + hg) * n;
-    c0 = x / per;
-    count = static_cast<int>((x + n - 1) / per - c0) + 1;
-    if (count == 1) return;                   // written by its CTA
+    const int64_t x = plan.before * R + static_cast<int64_t>(h * p.head_groups + hg) * n;
+    c0 = x / plan.per;
+    count = plan.whole ? 1 : static_cast<int>((x + n - 1) / plan.per - c0) + 1;
   }
+  grid_dep_wait();
+  if (!live || count == 1) return;            // one part: written by its CTA
   auto slot = [&](int i) { return (2 * (c0 + i) + (i == 0 ? 1 : 0)) * 8 * NT + head; };
   join_parts<D, W>(
       count, [&](int i) { return *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2); },
