@@ -11,8 +11,8 @@
 //   the tiles [c * per, (c + 1) * per) of it, per = ceil(tiles / CTAs), found on the device from
 //   kv_lens.  Every CTA streams the same number of tiles whatever the lengths are, and the launch
 //   does not depend on them (CUDA graphs).  A pair that lies in several CTAs leaves partial sums,
-//   which a second, dependent launch joins in a fixed order.  Where the pairs alone occupy the GPU
-//   evenly, each CTA takes one whole pair.
+//   which a second, dependent launch joins in a fixed order.  Many short pairs stay whole, one
+//   to a CTA.
 // * A producer warp issues TMA loads (K and V tile swizzled, their exponents as bulk copies);
 //   two pairs of consumer warps take the tiles in turn, each warp 32 of the 64 keys, and keep their own
 //   running maximum, sum and output until the pair ends, so tiles need no barrier among the warps.
@@ -146,11 +146,11 @@ struct Plan {
     live = __reduce_add_sync(0xffffffffu, live);
     most = __reduce_max_sync(0xffffffffu, most);
     per = (tiles * R + p.ctas - 1) / p.ctas;
-    // Pairs of nearly equal lengths that occupy a good part of the CTAs keep the memory busy without
-    // being split, and save the second segment of each CTA and the joining: 64 slots of about 1150 keys
-    // 21.8 us split, WHOLE64 whole; 48 windows of 4096 (head dim 64) 47.7 and WHOLEW.
+    // Short pairs that occupy a good part of the CTAs are not split: it saves each CTA a second segment and
+    // the joining.  Longer ones stream faster from all CTAs.  64 slots of about 270 / 540 / 1150 / 2300 keys,
+    // microseconds whole and split: 11.2, 13.4 / 13.7, 14.7 / 19.6, 19.0 / 35.4, 33.0.
     pairs = static_cast<int64_t>(live) * R;
-    whole = pairs <= p.ctas && 5 * pairs >= 2 * p.ctas && 4 * static_cast<int64_t>(most) * live <= 5 * tiles;
+    whole = pairs <= p.ctas && 5 * pairs >= 2 * p.ctas && most <= 12;
   }
 };
 
