@@ -235,45 +235,30 @@ __global__ void __launch_bounds__(kRope == kOddHalves ? 256 : 128, kRope == kOdd
   }
 }
 
-// One thread: 16 codes of one row of K and of V -> 32 bytes of bf16 each.
+// One thread: 8 codes of one row of K and of V, so that a warp's 16-byte stores lie side by side.
 template <int D>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8ReadArgs a) {
-  constexpr int L = D / 16;
+  constexpr int L = D / 8;
   grid_dep_launch();
   grid_dep_wait();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t r = i / L;
-  if (r >= static_cast<int64_t>(a.count) * a.hkv) return;
-  const int l = static_cast<int>(i - r * L);
-  const int n = static_cast<int>(r / a.hkv);
-  const int h = static_cast<int>(r - static_cast<int64_t>(n) * a.hkv);
+  const uint32_t r = blockIdx.x * (256 / L) + threadIdx.x / L, l = threadIdx.x % L;
+  if (r >= static_cast<uint32_t>(a.count) * a.hkv) return;   // below 2^31
+  const uint32_t n = r / static_cast<uint32_t>(a.hkv), h = r - n * a.hkv;
   const int64_t slot = a.slots[n];
-  uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+  uint2 raw[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
   float f[2] = {0.f, 0.f};
   if (slot >= 0 && slot < a.num_slots) {
     const int64_t row = ((slot >> 6) * a.hkv + h) * kPage + (slot & 63);
-    raw[0] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.k) + row * D + l * 16);
-    raw[1] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.v) + row * D + l * 16);
+    raw[0] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.k) + row * D + l * 8);
+    raw[1] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + row * D + l * 8);
     f[0] = pow2_of(static_cast<const int8_t*>(a.k_exp)[row]);
     f[1] = pow2_of(static_cast<const int8_t*>(a.v_exp)[row]);
   }
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const uint32_t four[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(w == 0 ? a.k_out : a.v_out) + r * D + l * 16);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4 t = e4m3x4_to_f32(four[2 * k + j]);
-        v[4 * j] = t.x * f[w];
-        v[4 * j + 1] = t.y * f[w];
-        v[4 * j + 2] = t.z * f[w];
-        v[4 * j + 3] = t.w * f[w];
-      }
-      dst[k] = pack8(v);
-    }
+    const float4 t = e4m3x4_to_f32(raw[w].x), u = e4m3x4_to_f32(raw[w].y);
+    const float v[8] = {t.x * f[w], t.y * f[w], t.z * f[w], t.w * f[w], u.x * f[w], u.y * f[w], u.z * f[w], u.w * f[w]};
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(w == 0 ? a.k_out : a.v_out) + static_cast<int64_t>(r) * D + l * 8) = pack8(v);
   }
 }
 
@@ -311,9 +296,9 @@ cudaError_t kv8_store(const Kv8StoreArgs& a, cudaStream_t stream) {
 
 cudaError_t kv8_read(const Kv8ReadArgs& a, cudaStream_t stream) {
   if (a.count == 0) return cudaSuccess;
-  const int64_t threads = static_cast<int64_t>(a.count) * a.hkv * (a.head_dim / 16);
-  const int64_t blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  const int64_t rows = static_cast<int64_t>(a.count) * a.hkv, per = 2048 / a.head_dim;
+  if (rows > 0x7fffffff) return cudaErrorInvalidValue;
+  const int64_t blocks = (rows + per - 1) / per;
   if (a.head_dim == 128)
     return launch_dependent(kv8_read_kernel<128>, dim3(static_cast<unsigned>(blocks)), 256, 0, stream, a);
   if (a.head_dim == 64)
