@@ -228,10 +228,12 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   // scratch from the caching allocator, used on the current stream only
   torch::Tensor scratch;
+  a.ctas = omni::kv8_decode_ctas(sms, static_cast<int>(hq / hkv), a.head_dim);
   if (!cu_q.has_value() || omni::kv8_few_tokens(a)) {
-    a.ctas = omni::kv8_decode_ctas(sms, static_cast<int>(hq / hkv), a.head_dim);
-    scratch = empty({omni::kv8_decode_scratch_floats(a.ctas, static_cast<int>(hq / hkv), a.head_dim)}, at::kFloat, k);
-    a.scratch = scratch.data_ptr<float>();
+    if (omni::kv8_decode_cluster(a) == 1) {
+      scratch = empty({omni::kv8_decode_scratch_floats(a.ctas, static_cast<int>(hq / hkv), a.head_dim)}, at::kFloat, k);
+      a.scratch = scratch.data_ptr<float>();
+    }
     check_launch(omni::kv8_decode(a, at::cuda::getCurrentCUDAStream()), "kv8_decode_attention");
   } else {
     torch::Tensor tiles;

@@ -30,19 +30,28 @@ cudaError_t ensure_smem_attr(int bytes) {
 // A launch that may start while the one before it on the stream still runs (programmatic dependent
 // launch): every thread of its kernel calls grid_dep_wait() before it reads memory or exits.
 template <class... Args>
-cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int block, int smem, cudaStream_t stream,
-                             const Args&... args) {
+cudaError_t launch_dependent_cluster(void (*kernel)(Args...), dim3 grid, int block, int smem, int cluster,
+                                     cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <class... Args>
+cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int block, int smem, cudaStream_t stream,
+                             const Args&... args) {
+  return launch_dependent_cluster(kernel, grid, block, smem, 1, stream, args...);
 }
 
 }  // namespace omni

@@ -63,7 +63,8 @@ struct Smem {
   static constexpr int kRedStride = D + 4;                      // floats; conflict-free float2 stores
   static constexpr int kRed = kExp + kStages * 2 * kPage;       // [warp][8 NT heads][D + 4]
   static constexpr int kMl = kRed + kWarps * 8 * NT * kRedStride * 4;   // [warp][8 NT][2] (m, l)
-  static constexpr int kBars = kMl + kWarps * 8 * NT * 8;
+  static constexpr int kSum = kMl + kWarps * 8 * NT * 8;              // [8 NT][2]: the CTA's own (m, l)
+  static constexpr int kBars = kSum + 8 * NT * 8;
   static constexpr int kBytes = kBars + 16 * kStages + 16 + 1024;
 };
 
@@ -86,6 +87,7 @@ struct Params {
   float* part_o;                                // [2 CTAs][8 NT][D]
   float* part_ml;                               // [2 CTAs][8 NT][2]
   int ctas;
+  int cluster;                                  // CTAs of a cluster that share a pair
   int* status;
 };
 
@@ -160,6 +162,8 @@ struct Walk {
   int i0, i1, n;          // this segment's tiles [i0, i1) of the pair's n
   int64_t left;
   int per_b;              // pairs per request
+  // tiles [i0, i1) of one pair
+  __device__ Walk(int b_, int r_, int n_, int i0_, int i1_) : b(b_), r(r_), i0(i0_), i1(i1_), n(n_), left(i1_ - i0_), per_b(0) {}
   // tiles [x, x + count) of all pairs', or pair x whole
   __device__ Walk(const Params& p, const Plan& plan, int64_t x, int64_t count, int R) {
     per_b = R;
@@ -245,6 +249,16 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ void store_row4(__nv_bfloat16* dst, const float4& x, float f) {
+  __nv_bfloat162 y[2] = {__floats2bfloat162_rn(x.x * f, x.y * f), __floats2bfloat162_rn(x.z * f, x.w * f)};
+  *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+}
+__device__ __forceinline__ float2 ld_dsmem_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 // Byte offset of 16-byte chunk c of row r in a swizzled tile (128-byte swizzle for 128-byte rows,
 // 64-byte swizzle for 64-byte rows).
 template <int D>
@@ -252,7 +266,28 @@ __device__ __forceinline__ int swz(int r, int c) {
   return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-template <int D, int NT>
+// What CTA blockIdx.x walks: a share of all tiles, or (kCluster) of its cluster's pair.
+template <bool kCluster>
+__device__ __forceinline__ Walk first_walk(const Params& p, int R, bool& any) {
+  if constexpr (kCluster) {
+    const int pair = blockIdx.x / p.cluster, rank = static_cast<int>(cluster_ctarank());
+    const int b = pair / R;
+    const int n = Span(p, b).tiles;
+    any = true;
+    return Walk(b, pair - b * R, n, static_cast<int>(static_cast<int64_t>(n) * rank / p.cluster),
+                static_cast<int>(static_cast<int64_t>(n) * (rank + 1) / p.cluster));
+  } else {
+    const Plan plan(p, R, 0);
+    const int64_t x = plan.whole ? static_cast<int64_t>(blockIdx.x) : blockIdx.x * plan.per;
+    any = plan.whole ? x < plan.pairs : x < plan.tiles * R;
+    if (!any) return Walk(0, 0, 0, 0, 0);
+    return Walk(p, plan, x, min(plan.per, plan.tiles * R - x), R);
+  }
+}
+
+// kCluster: the CTAs of a cluster take a pair's tiles in equal shares and join their sums through
+// distributed shared memory, so that there is no second launch.
+template <int D, int NT, bool kCluster>
 __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
     kv8_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Params p) {
   using S = Smem<D, NT>;
@@ -282,10 +317,9 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
   grid_dep_launch();   // after the wait: the joining launch may read kv_lens at once, and waits for the sums
 
   const int R = p.hkv * p.head_groups;
-  const Plan plan(p, R, 0);
-  const int64_t x0 = plan.whole ? static_cast<int64_t>(blockIdx.x) : blockIdx.x * plan.per;
-  if (plan.whole ? x0 >= plan.pairs : x0 >= plan.tiles * R) return;
-  Walk w(p, plan, x0, min(plan.per, plan.tiles * R - x0), R);
+  bool any;
+  Walk w = first_walk<kCluster>(p, R, any);
+  if (!any) return;
 
   if (warp == kWarps) {
     // ------------------------------------------------------------ producer
@@ -326,7 +360,8 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
     if (lane == 0)
       for (int64_t j = t > kStages ? t - kStages : 0; j < t; ++j)
         mbar_wait(&full[j % kStages], static_cast<uint32_t>((j / kStages) & 1), nullptr, p.status);
-    return;
+    __syncwarp();
+    if constexpr (!kCluster) return;
   }
 
   // -------------------------------------------------------------- consumers
@@ -337,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
   int s = 0;                      // their ring stage and phase
   uint32_t ph = 0;
   bool ok = true;
-  bool more = true;
+  bool more = warp < kWarps;
   while (more) {
     const Span sp(p, w.b);
     const int h = w.r / p.head_groups, hg = w.r - h * p.head_groups;
@@ -558,14 +593,12 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
         acc.w += x.w * f;
         ll += v.y * f;
       }
-      if (whole) {
+      if constexpr (kCluster) {
+        *reinterpret_cast<float4*>(red + head * S::kRedStride + d) = acc;   // the place of warp 0's share, read above
+        if (d == 0) reinterpret_cast<float2*>(smem + S::kSum)[head] = make_float2(mm, ll);
+      } else if (whole) {
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
-        uint2 two;
-        __nv_bfloat162 y = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-        two.x = *reinterpret_cast<uint32_t*>(&y);
-        y = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-        two.y = *reinterpret_cast<uint32_t*>(&y);
-        *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(w.b) * p.out_stride + static_cast<int64_t>(head0 + head) * D + d) = two;
+        store_row4(p.out + static_cast<int64_t>(w.b) * p.out_stride + static_cast<int64_t>(head0 + head) * D + d, acc, inv);
       } else {
         *reinterpret_cast<float4*>(p.part_o + (slot * 8 * NT + head) * D + d) = acc;
         if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * 8 * NT + head) * 2) = make_float2(mm, ll);
@@ -573,6 +606,35 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
     }
     asm volatile("bar.sync 1, 128;" ::: "memory");
     more = w.next(p);
+  }
+
+  if constexpr (kCluster) {
+    cluster_sync();
+    const int rank = static_cast<int>(cluster_ctarank());
+    const int h = w.r / p.head_groups, hg = w.r - h * p.head_groups;
+    const int head0 = h * p.group + hg * 8 * NT, items = min(8 * NT, p.group - hg * 8 * NT) * (D / 4);
+    for (int e = items * rank / p.cluster + static_cast<int>(threadIdx.x); e < items * (rank + 1) / p.cluster; e += kThreads) {
+      const int head = e / (D / 4), d = (e - head * (D / 4)) * 4;
+      const uint32_t sum_at = smem_u32(smem + S::kSum) + head * 8, o_at = smem_u32(red + head * S::kRedStride + d);
+      float mm = -INFINITY;
+      for (int u = 0; u < p.cluster; ++u) mm = fmaxf(mm, ld_dsmem_f2(dsmem_addr(sum_at, u)).x);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float ll = 0.f;
+#pragma unroll 4
+      for (int u = 0; u < p.cluster; ++u) {
+        const float2 v = ld_dsmem_f2(dsmem_addr(sum_at, u));
+        const float4 x = ld_dsmem_f4(dsmem_addr(o_at, u));
+        const float f = v.x == -INFINITY ? 1.f : ex2(v.x - mm);   // nothing (0), or a NaN to pass on
+        acc.x += x.x * f;
+        acc.y += x.y * f;
+        acc.z += x.z * f;
+        acc.w += x.w * f;
+        ll += v.y * f;
+      }
+      store_row4(p.out + static_cast<int64_t>(w.b) * p.out_stride + static_cast<int64_t>(head0 + head) * D + d, acc,
+                 ll == 0.f ? 0.f : 1.f / ll);
+    }
+    cluster_sync();   // no CTA leaves while another reads its shared memory
   }
 }
 
@@ -635,9 +697,15 @@ bool encode(CUtensorMap* map, const void* base, int d, int64_t rows) {
 template <int D, int NT>
 cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, cudaStream_t stream) {
   using S = Smem<D, NT>;
-  cudaError_t e = ensure_smem_attr<kv8_decode_kernel<D, NT>>(S::kBytes);
-  if (e != cudaSuccess) return e;
-  e = launch_dependent(kv8_decode_kernel<D, NT>, dim3(p.ctas), kThreads, S::kBytes, stream, tk, tv, p);
+  cudaError_t e;
+  if (p.cluster > 1) {
+    if ((e = ensure_smem_attr<kv8_decode_kernel<D, NT, true>>(S::kBytes)) != cudaSuccess) return e;
+    const int64_t grid = static_cast<int64_t>(p.batch) * p.hkv * p.head_groups * p.cluster;
+    return launch_dependent_cluster(kv8_decode_kernel<D, NT, true>, dim3(static_cast<unsigned>(grid)), kThreads, S::kBytes, p.cluster,
+                                    stream, tk, tv, p);
+  }
+  if ((e = ensure_smem_attr<kv8_decode_kernel<D, NT, false>>(S::kBytes)) != cudaSuccess) return e;
+  e = launch_dependent(kv8_decode_kernel<D, NT, false>, dim3(p.ctas), kThreads, S::kBytes, stream, tk, tv, p);
   if (e != cudaSuccess) return e;
   // a row's parts: about ctas / pairs; four warps for many parts, one where there are few and many rows
   const int64_t rows = static_cast<int64_t>(p.batch) * p.hq;
@@ -648,18 +716,33 @@ cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p
 
 }  // namespace
 
-// Chunks of few tokens: the decode kernel reads the context once per token (mostly out of L2), the chunk
-// kernel once, but expands it.  Microseconds, decode / chunk kernel, 32 / 4 heads of 128: 4 tokens on
-// 3000 keys 14 / 17, on 16,000 22 / 22, on 100,000 66 / 67; 8 tokens on 3000 keys 16 / 18, on
-// 100,000 118 / 69; 32 / 8 heads of 64: 4 tokens 13 / 12, 23 / 21, 84 / 87.
-bool kv8_few_tokens(const Kv8AttnArgs& a) {
-  const int64_t rows = a.q_rows, requests = a.batch;
-  return (rows <= 4 * requests && rows <= 512) || (rows <= 8 * requests && rows <= 64 && a.bt_pages <= 64);
-}
-
 int kv8_decode_ctas(int sm_count, int group, int head_dim) {
   return sm_count * (head_dim == 128 ? (group > 8 ? Smem<128, 2>::kCtas : Smem<128, 1>::kCtas)
                                      : (group > 8 ? Smem<64, 2>::kCtas : Smem<64, 1>::kCtas));
+}
+
+// CTAs of a cluster per pair, 1 for the launch over all tiles.  A cluster needs no joining launch and no
+// look-up of the other requests, but its shares follow its own request alone: taken where the pairs
+// with their clusters fit the GPU at once and no share can be long: 24 pages at the block table's width.  In
+// a graph, 32 / 4 heads of 128, microseconds by all tiles / by clusters: 1 request of 500 keys 7.3 / 5.7,
+// of 8000 (8 CTAs, 16 pages) 12.8 / 10.7, of 16,000 (31 pages) 15.1 / 16.5; 16 requests of 2000 (4 CTAs,
+// 8 pages) 13.3 / 11.2, of 4000 16.5 / 16.1, of 8000 28.0 / 28.6.
+int kv8_decode_cluster(const Kv8AttnArgs& a) {
+  const int group = a.hq / a.hkv, nt = group > 8 ? 2 : 1;
+  const int64_t pairs = static_cast<int64_t>(a.q_rows) * a.hkv * ((group + 8 * nt - 1) / (8 * nt));
+  for (int c = 8; c > 1; c >>= 1)
+    if (pairs * c <= a.ctas) return a.bt_pages <= 24 * c ? c : 1;
+  return 1;
+}
+
+// Chunks of few tokens: the decode kernel reads the context once per token (mostly out of L2), the chunk
+// kernel once, but expands it.  In a graph, 32 / 4 heads of 128, microseconds by the decode / chunk kernel: one request
+// of 4 tokens on 2000 keys 7.4 / 12.0, on 32,000 24 / 28; 8 on 8000 17 / 19; 16 on 4000 17 / 18; 8 requests of 2
+// tokens on 8000 35 / 40; of 4 on 2000 17 / 20, but on 4000, without clusters, 47 / 29.
+bool kv8_few_tokens(const Kv8AttnArgs& a) {
+  const int64_t rows = a.q_rows, requests = a.batch;
+  if (rows > 512) return false;
+  return rows <= 2 * requests || kv8_decode_cluster(a) > 1 || (requests == 1 && rows <= 4);
 }
 
 int64_t kv8_decode_scratch_floats(int ctas, int group, int head_dim) {
@@ -695,6 +778,7 @@ cudaError_t kv8_decode(const Kv8AttnArgs& a, cudaStream_t stream) {
   p.out = static_cast<__nv_bfloat16*>(a.out);
   p.out_stride = a.out_stride;
   p.ctas = a.ctas;
+  p.cluster = kv8_decode_cluster(a);
   p.part_o = a.scratch;
   p.part_ml = a.scratch + 2 * static_cast<int64_t>(a.ctas) * 8 * nt * a.head_dim;
   p.status = a.status;
