@@ -8,7 +8,9 @@
 //
 // kv8_read: rows by slot, as bf16 (exact).
 //
-// Both are bound by bytes.
+// Both are bound by bytes, the write also by its instructions (about 15 an element).  Measured: 8191
+// tokens of 32 + 2 x 4 heads of 128 with norm and M-RoPE, and the read of their rows: 44 us = 4.0 TB/s;
+// 130,000 rows of 2 x 4 heads read in 73 us = 5.5 TB/s (copy: 6.55).
 //
 // Reference counterpart: the fp8 KV-cache option of SGLang's token-to-KV pool behind
 // sglang_omni/engines/ar/sglang_backend/server_args_builder.py:10-35 (kv_cache_dtype there).
@@ -65,7 +67,6 @@ enum Rope : int {
 };
 template <int D, int kRope>
 __global__ void __launch_bounds__(kRope == kOddHalves ? 256 : 128, kRope == kOddHalves ? 2 : 6) kv8_store_kernel(const Kv8StoreArgs a, int passes) {
-  grid_dep_launch();
   constexpr int L = D / 16;         // lanes per head
   constexpr int HW = 32 / L;        // heads per warp and pass
   __shared__ float rows[kRope == kOddHalves ? 8 : 1][HW][D];   // partner exchange
@@ -81,6 +82,7 @@ __global__ void __launch_bounds__(kRope == kOddHalves ? 256 : 128, kRope == kOdd
   const int e0 = kRope == kHalves && rotates ? l * 8 : l * 16;
   const int e1 = kRope == kHalves && rotates ? l * 8 + half : l * 16 + 8;
   grid_dep_wait();
+  grid_dep_launch();   // not before the wait: a dependent grid would hold its shared memory while a GEMM still runs
   const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.qkv) + static_cast<int64_t>(tok) * a.qkv_stride;
   uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
   auto fetch = [&](int head) {
@@ -239,8 +241,8 @@ __global__ void __launch_bounds__(kRope == kOddHalves ? 256 : 128, kRope == kOdd
 template <int D>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8ReadArgs a) {
   constexpr int L = D / 8;
-  grid_dep_launch();
   grid_dep_wait();
+  grid_dep_launch();
   const uint32_t r = blockIdx.x * (256 / L) + threadIdx.x / L, l = threadIdx.x % L;
   if (r >= static_cast<uint32_t>(a.count) * a.hkv) return;   // below 2^31
   const uint32_t n = r / static_cast<uint32_t>(a.hkv), h = r - n * a.hkv;

@@ -27,6 +27,11 @@
 //   m is the running maximum of t (raised only when exceeded by 8), so what fp16 drops is below
 //   2^-31 of the largest contribution.  The softmax sum takes w_j * 2^-ev_j in fp32.
 //   q is scaled by a power of two to [2^9, 2^10) before it is rounded to fp16.
+//
+// Measured: 5 requests of 52,000 - 130,000 keys, 32 / 8 heads of 128: 204 - 210 us = 6.4 - 6.6 TB/s
+// (copy: 6.55); 64 slots of about 1150 keys, 32 / 4 heads, out of HBM: 22.7 us = 3.3 TB/s, of which about 8 us
+// are launches, look-ups and joining; 48 windows of 4096 keys, 32 / 8 heads of 64: 45 us = 4.5 TB/s; one
+// request of 517 keys: 6.3 us.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>

@@ -2,24 +2,33 @@
 //
 //   o_i = sum_j p_ij v_j,   p_i = softmax_j(q_i . k_j * scale) over the keys j visible to query i
 //
-// Bound by the tensor cores (4 D operations per visible pair) for long chunks, by the softmax's
-// exponentials next, and by the cache's bytes when a chunk has few rows.
+// Long chunks are bound by the tensor cores (4 D operations per visible pair) and, as much, by the
+// softmax's arithmetic on each score; chunks with few rows by the cache's bytes and latency.
 //
-// One CTA: two 128-row query tiles (GQA-packed: row r = token tok0 + r / G, head h G + r % G) that
-// share every 64-key block (one page), and a range of the blocks they see:
+// A CTA computes 128-row query tiles (GQA-packed: row r = token tok0 + r / G, head h G + r % G) over the
+// 64-key blocks (one page each) that they see:
 //
-// * Loader warps (4) read a block's codes and exponents into registers two blocks ahead, turn them
-//   into bf16 (exact: 4 significant bits times a power of two) and store them in the swizzled layout
-//   the tensor cores read; the cache's bytes cross HBM once per CTA at half of bf16's.
-// * One warp issues S = Q K^T and O += P V with S, P and O in tensor memory.  S has two buffers per
-//   tile: S of block j + 2 is issued once PV of block j is done, so the softmax never waits for the
-//   tensor core's latency, and P (bf16) takes the place of its S, so it never goes through shared memory.
-// * Two softmax warpgroups, one thread per row: running maximum (raised only when exceeded by 2^8),
-//   32-bit sums, O rescaled in tensor memory when the maximum is raised.
+// * Keys and values enter the tensor cores as bf16 (exact: 4 significant bits times a power of two) in the
+//   swizzled shared-memory layout.  Where several row tiles see the same blocks, a launch before expands
+//   each block once into global memory as it will lie in shared memory, and one loader thread fetches it
+//   by bulk copies; the CTA then works on two query tiles.  Otherwise eight loader warps expand the
+//   blocks themselves, reading two blocks ahead, for one query tile.
+// * One elected thread issues S = Q K^T and O += P V with S, P and O in tensor memory.  S has two
+//   buffers per tile, and between a PV and the S that takes its columns lie the other tile's two
+//   products, so neither the softmax nor the tensor core waits for a round trip.  P (bf16) takes
+//   the place of its S and never goes through shared memory.
+// * A softmax warpgroup per tile, one thread per row: running maximum (raised only when exceeded
+//   by 2^8), 32-bit sums, O rescaled in tensor memory when the maximum is raised.
 //
-// Chunks with few row tiles split the key blocks over the grid's third dimension; the partial
+// Chunks with few row tiles split the key blocks over the grid's second dimension; the partial
 // outputs are joined in order by a second, dependent launch.  The row tiles are found on the device
 // from cu_q, so a launch depends on sizes alone.
+//
+// Measured, 32 / 4 heads of 128: 2048 new tokens on 32,768 keys 905 us = 1253 TFLOP/s cold, 1047 us when
+// repeated under the power cap (cuBLAS bf16: 1627 and 1391); 8 chunks of 100 - 1024 tokens on up to 2500
+// keys 172 - 183 us.  The two-tile loop takes about 1600 cycles a block: 1024 of tensor-core arithmetic
+// (1280 with the shared-memory reads of 64-key S products), 1024 of exponentials.  Sixteen softmax
+// warps (two threads a row) took 987 us, persistent CTAs that fetch the next tile early 949.
 //
 // A key whose K or V row is marked as not finite enters as a NaN key row and a zero value row: its
 // scores are NaN for the queries that see it, and masked by selection for those that do not.
@@ -321,8 +330,8 @@ struct Blocks {
 // [request][page][KV head], as they will lie in shared memory).
 template <int D>
 __global__ void __launch_bounds__(kExpandThreads) kv8_expand_kernel(const Params p) {
-  grid_dep_launch();
   grid_dep_wait();
+  grid_dep_launch();
   const int req = blockIdx.y, h = blockIdx.z;
   const int n = p.cu_q[req + 1] - p.cu_q[req];
   const int kv_len = max(0, min(p.kv_lens[req], p.bt_pages * kPage));
@@ -357,8 +366,8 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  grid_dep_launch();
   grid_dep_wait();
+  grid_dep_launch();
 
   // Row tile and KV head of this CTA.  The grid hands CTAs out in order, and the last to start should be
   // short: requests by falling context (up to 32 of them; by position in the batch beyond), each

@@ -197,7 +197,8 @@ def kv8_prefill_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.T
                           scale: float | None = None, window: int = 0, sinks: int = 0,
                           out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of each request's new tokens (rows cu_q[b] .. cu_q[b + 1] of q, the last of
-    its ``kv_lens[b]`` keys).  q: [T, >= Hq * D] rows.  The new tokens' keys are in the cache already."""
+    its ``kv_lens[b]`` keys).  q: [T, >= Hq * D] rows.  The new tokens' keys are in the cache already.
+    Rows from cu_q[-1] on are unspecified."""
     scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
     if q.is_cuda:
         if _check.enabled():
