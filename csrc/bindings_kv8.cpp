@@ -192,6 +192,7 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
     a.cu_q = int_ptr(*cu_q, k, "cu_q");
     TORCH_CHECK(cu_q->numel() == B + 1, "cu_q needs one entry more than kv_lens");
   } else {
+    TORCH_CHECK(T * block_table.size(1) < (int64_t{1} << 31), "block_table is too large");
     TORCH_CHECK(T == B, "decode takes one query row per request: " + num(T) + " rows, " + num(B) + " requests");
   }
   torch::Tensor out = out_.has_value() ? *out_ : empty({T, hq * head_dim}, at::kBFloat16, k);

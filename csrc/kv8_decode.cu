@@ -124,23 +124,16 @@ struct Span {
   __device__ int tile(int i) const { return i < sink_tiles ? i : first + i - sink_tiles; }
 };
 
-__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
-}
-
 // How the tiles are dealt out (whole warp; the same in every warp of both launches).
 struct Plan {
-  int64_t tiles;          // of one (KV head, head group), over all requests
-  int64_t before;         // of them, in the requests before `stop`
+  int tiles;              // of one (KV head, head group), over all requests (below 2^31)
+  int before;             // of them, in the requests before `stop`
   int64_t per;            // tiles of a CTA
   int64_t pairs;          // with a visible key
   bool whole;             // a pair per CTA instead
   __device__ Plan(const Params& p, int R, int stop) {
     const int lane = threadIdx.x & 31;
-    int64_t all = 0, head = 0;
-    int live = 0, most = 0;
+    int all = 0, head = 0, live = 0, most = 0;
     for (int b = lane; b < p.batch; b += 32) {
       const int n = Span(p, b).tiles;
       all += n;
@@ -148,11 +141,11 @@ struct Plan {
       live += n > 0;
       most = max(most, n);
     }
-    tiles = warp_sum64(all);
-    before = warp_sum64(head);
+    tiles = __reduce_add_sync(0xffffffffu, all);
+    before = __reduce_add_sync(0xffffffffu, head);
     live = __reduce_add_sync(0xffffffffu, live);
     most = __reduce_max_sync(0xffffffffu, most);
-    per = (tiles * R + p.ctas - 1) / p.ctas;
+    per = (static_cast<int64_t>(tiles) * R + p.ctas - 1) / p.ctas;
     // Short pairs that occupy a good part of the CTAs are not split: it saves each CTA a second segment and
     // the joining.  Longer ones stream faster from all CTAs.  64 slots of about 270 / 540 / 1150 / 2300 keys,
     // microseconds whole and split: 11.2, 13.4 / 13.7, 14.7 / 19.6, 19.0 / 35.4, 33.0.
@@ -174,18 +167,18 @@ struct Walk {
     per_b = R;
     left = count;
     const int lane = threadIdx.x & 31;
-    int64_t cum = 0;
+    int cum = 0;
     b = 0;
     for (int base = 0; base < p.batch; base += 32) {
       const int mine = base + lane < p.batch ? Span(p, base + lane).tiles : 0;
-      const int64_t weight = plan.whole ? (mine > 0 ? 1 : 0) : mine;
-      int64_t inc = weight;
+      const int weight = plan.whole ? (mine > 0 ? 1 : 0) : mine;
+      int inc = weight;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, inc, d);
+        const int up = __shfl_up_sync(0xffffffffu, inc, d);
         if (lane >= d) inc += up;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, (cum + inc) * R > x);
+      const unsigned past = __ballot_sync(0xffffffffu, static_cast<int64_t>(cum + inc) * R > x);
       if (past != 0) {
         const int at = __ffs(past) - 1;
         b = base + at;
@@ -195,13 +188,14 @@ struct Walk {
       }
       cum += __shfl_sync(0xffffffffu, inc, 31);
     }
-    const int64_t rel = x - cum * R;
+    const int64_t rel = x - static_cast<int64_t>(cum) * R;
     if (plan.whole) {
       r = static_cast<int>(rel);
       i0 = 0;
       left = n;
     } else {
-      r = static_cast<int>(rel / n);
+      // rel < n R; 32-bit division where that fits
+      r = rel < 0x7fffffff ? static_cast<int>(rel) / n : static_cast<int>(rel / n);
       i0 = static_cast<int>(rel - static_cast<int64_t>(r) * n);
     }
     i1 = static_cast<int>(min(static_cast<int64_t>(n), i0 + left));
@@ -284,9 +278,10 @@ __device__ __forceinline__ Walk first_walk(const Params& p, int R, bool& any) {
   } else {
     const Plan plan(p, R, 0);
     const int64_t x = plan.whole ? static_cast<int64_t>(blockIdx.x) : blockIdx.x * plan.per;
-    any = plan.whole ? x < plan.pairs : x < plan.tiles * R;
+    const int64_t all = static_cast<int64_t>(plan.tiles) * R;
+    any = plan.whole ? x < plan.pairs : x < all;
     if (!any) return Walk(0, 0, 0, 0, 0);
-    return Walk(p, plan, x, min(plan.per, plan.tiles * R - x), R);
+    return Walk(p, plan, x, min(plan.per, all - x), R);
   }
 }
 
@@ -660,7 +655,7 @@ __global__ void __launch_bounds__(128) kv8_decode_join_kernel(const Params p) {
   int64_t c0 = 0;
   int count = 0;
   if (n > 0) {
-    const int64_t x = plan.before * R + static_cast<int64_t>(h * p.head_groups + hg) * n;
+    const int64_t x = static_cast<int64_t>(plan.before) * R + static_cast<int64_t>(h * p.head_groups + hg) * n;
     c0 = x / plan.per;
     count = plan.whole ? 1 : static_cast<int>((x + n - 1) / plan.per - c0) + 1;
   }
@@ -746,7 +741,7 @@ int kv8_decode_cluster(const Kv8AttnArgs& a) {
 // tokens on 8000 35 / 40; of 4 on 2000 17 / 20, but on 4000, without clusters, 47 / 29.
 bool kv8_few_tokens(const Kv8AttnArgs& a) {
   const int64_t rows = a.q_rows, requests = a.batch;
-  if (rows > 512) return false;
+  if (rows > 512 || rows * a.bt_pages >= (int64_t{1} << 31)) return false;
   return rows <= 2 * requests || kv8_decode_cluster(a) > 1 || (requests == 1 && rows <= 4);
 }
 
