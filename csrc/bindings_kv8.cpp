@@ -231,7 +231,7 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
   torch::Tensor scratch;
   a.ctas = omni::kv8_decode_ctas(sms, static_cast<int>(hq / hkv), a.head_dim);
   if (!cu_q.has_value() || omni::kv8_few_tokens(a)) {
-    if (omni::kv8_decode_cluster(a) == 1) {
+    if (omni::kv8_decode_cluster(a) == 0) {
       scratch = empty({omni::kv8_decode_scratch_floats(a.ctas, static_cast<int>(hq / hkv), a.head_dim)}, at::kFloat, k);
       a.scratch = scratch.data_ptr<float>();
     }

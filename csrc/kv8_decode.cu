@@ -36,6 +36,7 @@
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -698,7 +699,7 @@ template <int D, int NT>
 cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const Params& p, cudaStream_t stream) {
   using S = Smem<D, NT>;
   cudaError_t e;
-  if (p.cluster > 1) {
+  if (p.cluster > 0) {
     if ((e = ensure_smem_attr<kv8_decode_kernel<D, NT, true>>(S::kBytes)) != cudaSuccess) return e;
     const int64_t grid = static_cast<int64_t>(p.batch) * p.hkv * p.head_groups * p.cluster;
     return launch_dependent_cluster(kv8_decode_kernel<D, NT, true>, dim3(static_cast<unsigned>(grid)), kThreads, S::kBytes, p.cluster,
@@ -721,18 +722,22 @@ int kv8_decode_ctas(int sm_count, int group, int head_dim) {
                                      : (group > 8 ? Smem<64, 2>::kCtas : Smem<64, 1>::kCtas));
 }
 
-// CTAs of a cluster per pair, 1 for the launch over all tiles.  A cluster needs no joining launch and no
+// CTAs of a cluster per pair, 0 for the launch over all tiles.  A cluster needs no joining launch and no
 // look-up of the other requests, but its shares follow its own request alone: taken where the pairs
-// with their clusters fit the GPU at once and no share can be long: 24 pages at the block table's width.  In
-// a graph, 32 / 4 heads of 128, microseconds by all tiles / by clusters: 1 request of 500 keys 7.3 / 5.7,
-// of 8000 (8 CTAs, 16 pages) 12.8 / 10.7, of 16,000 (31 pages) 15.1 / 16.5; 16 requests of 2000 (4 CTAs,
-// 8 pages) 13.3 / 11.2, of 4000 16.5 / 16.1, of 8000 28.0 / 28.6.
+// with their clusters fit the GPU at once and no share can be long: 24 tiles at what the block table's width and
+// the window allow.  In a graph, 32 / 4 heads of 128, microseconds by all tiles / by clusters: 1 request of
+// 500 keys 7.3 / 5.7, of 8000 (8 CTAs, 16 tiles) 12.8 / 10.7, of 16,000 (31 tiles) 15.1 / 16.5; 16 requests of
+// 2000 (4 CTAs, 8 tiles) 13.3 / 11.2, of 4000 16.5 / 16.1, of 8000 28.0 / 28.6; one CTA a pair, 64 slots of 1280
+// 22.7 / 20.9, of 2000 31.3 / 30.3, of 3000 40.5 / 41.4; nearly a CTA for each pair, 100 slots of 3000 56.8 / 51.2, of
+// 2200 - 4500 64.7 / 64.5.
 int kv8_decode_cluster(const Kv8AttnArgs& a) {
   const int group = a.hq / a.hkv, nt = group > 8 ? 2 : 1;
   const int64_t pairs = static_cast<int64_t>(a.q_rows) * a.hkv * ((group + 8 * nt - 1) / (8 * nt));
-  for (int c = 8; c > 1; c >>= 1)
-    if (pairs * c <= a.ctas) return a.bt_pages <= 24 * c ? c : 1;
-  return 1;
+  int64_t tiles = a.bt_pages;
+  if (a.window > 0) tiles = std::min<int64_t>(tiles, (static_cast<int64_t>(a.window) + 63) / 64 + 1 + (static_cast<int64_t>(a.sinks) + 63) / 64);
+  for (int c = 8; c > 0; c >>= 1)
+    if (pairs * c <= a.ctas) return tiles <= (c == 1 && 4 * pairs >= 3 * a.ctas ? 64 : 24 * c) ? c : 0;
+  return 0;
 }
 
 // Chunks of few tokens: the decode kernel reads the context once per token (mostly out of L2), the chunk
@@ -742,7 +747,7 @@ int kv8_decode_cluster(const Kv8AttnArgs& a) {
 bool kv8_few_tokens(const Kv8AttnArgs& a) {
   const int64_t rows = a.q_rows, requests = a.batch;
   if (rows > 512 || rows * a.bt_pages >= (int64_t{1} << 31)) return false;
-  return rows <= 2 * requests || kv8_decode_cluster(a) > 1 || (requests == 1 && rows <= 4);
+  return rows <= 2 * requests || kv8_decode_cluster(a) > 0 || (requests == 1 && rows <= 4);
 }
 
 int64_t kv8_decode_scratch_floats(int ctas, int group, int head_dim) {

@@ -252,7 +252,7 @@ int kv8_prefill_splits(const Kv8AttnArgs& a, int sm_count);   // after `tiles` i
 int64_t kv8_prefill_scratch_floats(const Kv8AttnArgs& a);     // after `splits` is set
 cudaError_t kv8_prefill(const Kv8AttnArgs& a, cudaStream_t stream);
 int kv8_decode_ctas(int sm_count, int group, int head_dim);
-int kv8_decode_cluster(const Kv8AttnArgs& a);           // after `ctas` is set; > 1: no scratch
+int kv8_decode_cluster(const Kv8AttnArgs& a);           // after `ctas` is set; > 0: no scratch
 int64_t kv8_decode_scratch_floats(int ctas, int group, int head_dim);
 cudaError_t kv8_decode(const Kv8AttnArgs& a, cudaStream_t stream);   // cu_q: each row its own request
 bool kv8_few_tokens(const Kv8AttnArgs& a);   // chunks that kv8_decode takes (after `ctas` is set)
