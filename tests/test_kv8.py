@@ -429,3 +429,63 @@ def test_refusals():
     assert ops.kv8_prefill_attention(none, cache, bt, i32(0, 0, 0), i32(0, 5), **ok).shape == (0, hq * d)
     assert ops.kv8_read(cache, i32())[0].shape == (0, hkv, d)
     assert ops.kv8_store(torch.zeros(0, 8 * d, device="cuda", dtype=torch.bfloat16), cache, i32(), **ok).shape == (0, hq * d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,width,top", [
+    (20, 8, 300), (40, 8, 200), (80, 8, 150), (150, 8, 120),      # clusters of 4, 2, 1 CTAs a pair; shares of all tiles
+    (60, 70, 300), (60, 70, 1500), (3, 300, 2500)])               # wide tables: short pairs whole; split; few and long
+@pytest.mark.parametrize("d", [64, 128])
+def test_decode_ways_of_sharing(batch, width, top, d):
+    """Every way in which the tiles are dealt out, with empty, short and unequal contexts."""
+    hq, hkv = 8, 4
+    kv_lens = [0 if b % 9 == 4 else 1 + (b * 37) % top for b in range(batch)]
+    pages = sum((n + 63) // 64 for n in kv_lens) + 2
+    cache = make_cache(pages, hkv, d, "cuda", seed=8)
+    bt = make_table(kv_lens, pages, seed=8, width=max(width, (top + 63) // 64)).cuda()
+    q = torch.randn(batch, hq * d, generator=torch.Generator().manual_seed(12)).bfloat16().cuda()
+    kl = torch.tensor(kv_lens, dtype=torch.int32, device="cuda")
+    for window, sinks in ((0, 0), (90, 5)):
+        out = ops.kv8_decode_attention(q, cache, bt, kl, hq, hkv, d, window=window, sinks=sinks)
+        check_attention(out, q, cache, bt, [1] * batch, kv_lens, hq, hkv, d, d ** -0.5, window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(16, 2, 128), (14, 2, 128), (33, 1, 128), (2, 2, 64), (40, 8, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (64, 64), (150, 100), (70, 3)])
+def test_chunk_expanded(hq, hkv, d, window, sinks):
+    """Chunks of several row tiles per request (the blocks are expanded by a launch of their own), with windows
+    that begin inside, at and between blocks, and a request without new tokens."""
+    q_lens = [300, 0, 257, 290]
+    kv_lens = [300, 77, 700, 291]
+    if hq // hkv < 4:      # more tokens to a row tile
+        q_lens, kv_lens = [600, 0, 530, 520], [600, 77, 1100, 521]
+    pages = sum((n + 63) // 64 for n in kv_lens) + 2
+    cache = make_cache(pages, hkv, d, "cuda", seed=9)
+    bt = make_table(kv_lens, pages, seed=9).cuda()
+    q = torch.randn(sum(q_lens), hq * d, generator=torch.Generator().manual_seed(13)).bfloat16().cuda()
+    cu = torch.tensor([sum(q_lens[:i]) for i in range(len(q_lens) + 1)], dtype=torch.int32, device="cuda")
+    kl = torch.tensor(kv_lens, dtype=torch.int32, device="cuda")
+    out = ops.kv8_prefill_attention(q, cache, bt, cu, kl, hq, hkv, d, window=window, sinks=sinks)
+    check_attention(out, q, cache, bt, q_lens, kv_lens, hq, hkv, d, d ** -0.5, window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40, 300])
+def test_queries_that_are_not_finite(new):
+    """A query with an infinity or a NaN gives NaN, and nothing to its neighbours (decode, chunk and expanded chunk)."""
+    hq, hkv, d, n = 8, 2, 128, 500
+    cache = make_cache(10, hkv, d, "cuda", seed=10)
+    bt = make_table([n], 10, seed=10).cuda()
+    q = torch.randn(new, hq * d, generator=torch.Generator().manual_seed(14)).bfloat16()
+    clean = q.clone()
+    for t in {0, new // 2}:
+        q[t, 3] = float("inf")                    # head 0
+        q[t, 5 * d + 7] = float("nan")            # head 5
+    cu, kl = torch.tensor([0, new], dtype=torch.int32).cuda(), torch.tensor([n], dtype=torch.int32).cuda()
+    got = ops.kv8_prefill_attention(q.cuda(), cache, bt, cu, kl, hq, hkv, d).cpu().view(new, hq, d)
+    want = ops.kv8_prefill_attention(clean.cuda(), cache, bt, cu, kl, hq, hkv, d).cpu().view(new, hq, d)
+    hit = torch.zeros(new, hq, dtype=torch.bool)
+    for t in {0, new // 2}:
+        hit[t, 0] = hit[t, 5] = True
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], want[~hit])
