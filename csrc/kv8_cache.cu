@@ -9,7 +9,7 @@
 // kv8_read: rows by slot, as bf16 (exact).
 //
 // Both are bound by bytes, the write also by its instructions (about 15 an element).  Measured: 8191
-// tokens of 32 + 2 x 4 heads of 128 with norm and M-RoPE, and the read of their rows: 44 us = 4.0 TB/s;
+// tokens of 32 + 2 x 4 heads of 128 with norm and M-RoPE 36 us = 4.4 TB/s;
 // 130,000 rows of 2 x 4 heads read in 73 us = 5.5 TB/s (copy: 6.55).
 //
 // Reference counterpart: the fp8 KV-cache option of SGLang's token-to-KV pool behind
@@ -66,7 +66,7 @@ enum Rope : int {
   kOddHalves,   // halves of any size: partners through shared memory
 };
 template <int D, int kRope>
-__global__ void __launch_bounds__(kRope == kOddHalves ? 256 : 128, kRope == kOddHalves ? 2 : 6) kv8_store_kernel(const Kv8StoreArgs a, int passes) {
+__global__ void __launch_bounds__(kRope == kOddHalves ? 256 : 128, kRope == kOddHalves ? 2 : 7) kv8_store_kernel(const Kv8StoreArgs a, int passes) {
   constexpr int L = D / 16;         // lanes per head
   constexpr int HW = 32 / L;        // heads per warp and pass
   __shared__ float rows[kRope == kOddHalves ? 8 : 1][HW][D];   // partner exchange

@@ -28,7 +28,8 @@
 // repeated under the power cap (cuBLAS bf16: 1627 and 1391); 8 chunks of 100 - 1024 tokens on up to 2500
 // keys 172 - 183 us.  The two-tile loop takes about 1600 cycles a block: 1024 of tensor-core arithmetic
 // (1280 with the shared-memory reads of 64-key S products), 1024 of exponentials.  Sixteen softmax
-// warps (two threads a row) took 987 us, persistent CTAs that fetch the next tile early 949.
+// warps (two threads a row) took 987 us, weights at the last maximum beside the block's own 949, persistent CTAs
+// that fetch the next tile early 949.
 //
 // A key whose K or V row is marked as not finite enters as a NaN key row and a zero value row: its
 // scores are NaN for the queries that see it, and masked by selection for those that do not.
