@@ -760,7 +760,8 @@ cudaError_t launch(const Params& p, int64_t tiles, cudaStream_t stream) {
 
 int64_t row_tiles(int64_t q_rows, int batch, int group, bool expanded) {
   const int64_t step = tiles_of(expanded) * (kRows / group);
-  return std::min(q_rows, q_rows / step + batch);     // each request ends in at most one partial tile
+  // n tokens make at most (n - 1) / step + 1 tiles
+  return std::min(q_rows, std::max<int64_t>(0, q_rows - batch) / step + batch);
 }
 
 }  // namespace
