@@ -51,14 +51,16 @@ using namespace kv8;
 
 constexpr int kRows = 128;                 // rows of a query tile
 constexpr int kBN = kPage;                 // keys of a block
-constexpr int kStages = 5;
+// Ring stages of expanded blocks, and of blocks still in codes (where the CTA expands them itself).
+constexpr int stages(bool expanded) { return expanded ? 5 : 4; }
+constexpr int kRaw = 4;
 constexpr int kExpandThreads = 128;
 // Two query tiles and one loader warp where the tiles come expanded; one query tile and eight loader
 // warps where the loaders expand them (the few rows of such a launch do not fill a second tile, and four
 // loader warps took 3000 cycles a block, twice the softmax's time).
 constexpr int tiles_of(bool expanded) { return expanded ? 2 : 1; }
 constexpr int load_warps(bool expanded) { return expanded ? 1 : 8; }
-constexpr int threads(bool expanded) { return 32 * (4 * tiles_of(expanded) + load_warps(expanded) + 1); }
+constexpr int threads(bool expanded) { return 32 * (4 * tiles_of(expanded) + load_warps(expanded) + (expanded ? 1 : 2)); }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.0f;             // log2 units
 // Of every 8 pairs of scores, those whose exponential runs on the FMA pipe instead of the special-function
@@ -68,16 +70,19 @@ constexpr int kTmemCols = 512;             // S/P: tile x buffer x 64, O: tile x
 constexpr int kRegionQ = kRows * 128;      // 64 columns of a query tile
 constexpr int kRegionK = kBN * 128;        // 64 columns of a block
 
-template <int D>
+template <int D, bool kExpanded>
 struct Smem {
   static constexpr int kQ = 0;
   static constexpr int kQBytes = kRows * D * 2;
-  static constexpr int kKV = 2 * kQBytes;
+  static constexpr int kKV = tiles_of(kExpanded) * kQBytes;
   static constexpr int kKBytes = kBN * D * 2;
-  static constexpr int kBars = kKV + kStages * 2 * kKBytes;
-  static constexpr int kBytes = kBars + 256 + 1024;
+  static constexpr int kRaw0 = kKV + stages(kExpanded) * 2 * kKBytes;
+  static constexpr int kCodes = kBN * D;
+  static constexpr int kRawBytes = 2 * kCodes + 2 * kBN;         // K codes, V codes, exponents of K, of V
+  static constexpr int kBars = kRaw0 + (kExpanded ? 0 : kRaw * kRawBytes);
+  static constexpr int kBytes = kBars + 512 + 1024;
 };
-static_assert(Smem<128>::kBytes <= 232448, "shared memory exceeds 227 KB");
+static_assert(Smem<128, true>::kBytes <= 232448 && Smem<128, false>::kBytes <= 232448, "shared memory exceeds 227 KB");
 
 struct Params {
   const __nv_bfloat16* q;
@@ -254,9 +259,9 @@ struct Share {
 
 template <int N>
 __device__ __forceinline__ uint32_t load_bytes(const int8_t* p) {
-  if constexpr (N == 4) return __ldg(reinterpret_cast<const uint32_t*>(p));
-  if constexpr (N == 2) return __ldg(reinterpret_cast<const uint16_t*>(p));
-  return __ldg(reinterpret_cast<const uint8_t*>(p));
+  if constexpr (N == 4) return *reinterpret_cast<const uint32_t*>(p);
+  if constexpr (N == 2) return *reinterpret_cast<const uint16_t*>(p);
+  return *reinterpret_cast<const uint8_t*>(p);
 }
 
 template <int D, int TH>
@@ -264,18 +269,16 @@ struct Part {
   static constexpr int CH = D / 16;              // 16-code chunks of a row
   static constexpr int N = kBN * CH / TH;        // rows per thread
   Share<N> x;
-  // Thread `tid` of TH reads its share of the block whose first row is row0.
-  __device__ __forceinline__ void fetch(const Params& p, int64_t row0, int tid) {
-    row0 += tid / CH * N;
-    const uint8_t* k = p.k + row0 * D + tid % CH * 16;
-    const uint8_t* v = p.v + row0 * D + tid % CH * 16;
+  // Thread `tid` of TH reads its share of a block's codes and exponents.
+  __device__ __forceinline__ void fetch(const uint8_t* k, const uint8_t* v, const int8_t* ke, const int8_t* ve, int tid) {
+    const int r0 = tid / CH * N, at = r0 * D + tid % CH * 16;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      x.k[i] = __ldg(reinterpret_cast<const uint4*>(k + i * D));
-      x.v[i] = __ldg(reinterpret_cast<const uint4*>(v + i * D));
+      x.k[i] = *reinterpret_cast<const uint4*>(k + at + i * D);
+      x.v[i] = *reinterpret_cast<const uint4*>(v + at + i * D);
     }
-    x.ke = load_bytes<N>(p.k_exp + row0);
-    x.ve = load_bytes<N>(p.v_exp + row0);
+    x.ke = load_bytes<N>(ke + r0);
+    x.ve = load_bytes<N>(ve + r0);
   }
   // Expands it into the block's K and V tiles (the tensor core's swizzled layout); rows from `left`
   // on lie past the context: their values become zeros (their scores are masked).
@@ -342,15 +345,18 @@ __global__ void __launch_bounds__(kExpandThreads) kv8_expand_kernel(const Params
   const int i = bl.at(blockIdx.x);
   const int page = checked_page(p.block_table[static_cast<int64_t>(req) * p.bt_stride + i], p.num_pages);
   Part<D, kExpandThreads> part;
-  part.fetch(p, (static_cast<int64_t>(page) * p.hkv + h) * kPage, threadIdx.x);
-  uint8_t* dst = p.tiles + ((static_cast<int64_t>(req) * p.bt_pages + i) * p.hkv + h) * (2 * Smem<D>::kKBytes);
-  part.store(dst, dst + Smem<D>::kKBytes, kv_len - i * kPage, threadIdx.x);
+  const int64_t row0 = (static_cast<int64_t>(page) * p.hkv + h) * kPage;
+  part.fetch(p.k + row0 * D, p.v + row0 * D, p.k_exp + row0, p.v_exp + row0, threadIdx.x);
+  constexpr int kTile = Smem<D, true>::kKBytes;
+  uint8_t* dst = p.tiles + ((static_cast<int64_t>(req) * p.bt_pages + i) * p.hkv + h) * (2 * kTile);
+  part.store(dst, dst + kTile, kv_len - i * kPage, threadIdx.x);
 }
 
 // kExpanded: the K / V tiles come ready from kv8_expand_kernel by bulk copies.
 template <int D, bool kExpanded>
 __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(const Params p) {
-  using S = Smem<D>;
+  using S = Smem<D, kExpanded>;
+  constexpr int kStages = stages(kExpanded);
   constexpr int kTiles = tiles_of(kExpanded), kLoadWarps = load_warps(kExpanded);
   constexpr int kLoad0 = 4 * kTiles, kMmaWarp = kLoad0 + kLoadWarps;
   extern __shared__ uint8_t raw[];
@@ -364,7 +370,9 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
   uint64_t* pv_done = p_full + 4;              // [2] tile
   uint64_t* o_full = pv_done + 2;              // [2] tile: the last PV
   uint64_t* drain = o_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* raw_full = drain + 1;              // [kRaw]
+  uint64_t* raw_empty = raw_full + kRaw;       // [kRaw]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + kRaw);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   grid_dep_wait();
@@ -430,6 +438,10 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
       mbar_init(&kv_full[i], kLoadWarps);
       mbar_init(&kv_empty[i], 1);
     }
+    for (int i = 0; i < kRaw; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], kLoadWarps);
+    }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
@@ -471,34 +483,46 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
     } else {
       constexpr int TH = 32 * kLoadWarps;
       const int tid = threadIdx.x - 32 * kLoad0;
-      const int* table = p.block_table + static_cast<int64_t>(req) * p.bt_stride;
-      auto page_of = [&](int j) { return j < nb ? checked_page(table[block_of(j)], p.num_pages) : 0; };
-      auto fetch = [&](int j, int page, Part<D, TH>& x) {
-        if (j < nb) x.fetch(p, (static_cast<int64_t>(page) * p.hkv + h) * kPage, tid);
-      };
-      Part<D, TH> buf[3];                       // blocks j, j + 1, j + 2
-      bool ok = true;
-      int page = page_of(2);
-      fetch(0, page_of(0), buf[0]);
-      fetch(1, page_of(1), buf[1]);
-      auto put = [&](int j, Part<D, TH>& cur, Part<D, TH>& far) {
-        fetch(j + 2, page, far);
-        page = page_of(j + 3);
-        if (j >= kStages) ok = warp_wait(&kv_empty[stage], phase, abort_flag, p.status, 41);
-        if (!ok) return;
+      for (int j = 0; j < nb; ++j) {
+        const int rs = j % kRaw;
+        if (!warp_wait(&raw_full[rs], (j / kRaw) & 1, abort_flag, p.status, 49)) break;
+        const uint8_t* k = smem + S::kRaw0 + rs * S::kRawBytes;
+        const int8_t* e = reinterpret_cast<const int8_t*>(k + 2 * S::kCodes);
+        Part<D, TH> part;
+        part.fetch(k, k + S::kCodes, e, e + kBN, tid);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&raw_empty[rs]);
+        if (j >= kStages && !warp_wait(&kv_empty[stage], phase, abort_flag, p.status, 41)) break;
         uint8_t* dk = smem + S::kKV + stage * 2 * S::kKBytes;
-        cur.store(dk, dk + S::kKBytes, kv_len - block_of(j) * kPage, tid);
+        part.store(dk, dk + S::kKBytes, kv_len - block_of(j) * kPage, tid);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&kv_full[stage]);
         if (++stage == kStages) stage = 0, phase ^= 1;
-      };
-      for (int j = 0; j < nb && ok; j += 3) {
-        put(j, buf[0], buf[2]);
-        if (j + 1 < nb && ok) put(j + 1, buf[1], buf[0]);
-        if (j + 2 < nb && ok) put(j + 2, buf[2], buf[1]);
       }
     }
+  } else if (warp == kMmaWarp + 1) {
+    // ------------------------------------------------------------ copies of the blocks' codes
+    if (elect_one()) {
+      const int* table = p.block_table + static_cast<int64_t>(req) * p.bt_stride;
+      auto page_of = [&](int j) { return j < nb ? checked_page(table[block_of(j)], p.num_pages) : 0; };
+      int page = page_of(0), j = 0;
+      for (; j < nb; ++j) {
+        const int rs = j % kRaw;
+        const int64_t row0 = (static_cast<int64_t>(page) * p.hkv + h) * kPage;
+        page = page_of(j + 1);
+        if (j >= kRaw && !mbar_wait(&raw_empty[rs], (j / kRaw - 1) & 1, abort_flag, p.status, kWaitTimeoutNs, kStatusWaitSite + 50)) break;
+        uint8_t* dst = smem + S::kRaw0 + rs * S::kRawBytes;
+        mbar_arrive_expect_tx(&raw_full[rs], S::kRawBytes);
+        bulk_copy(dst, p.k + row0 * D, S::kCodes, &raw_full[rs]);
+        bulk_copy(dst + S::kCodes, p.v + row0 * D, S::kCodes, &raw_full[rs]);
+        bulk_copy(dst + 2 * S::kCodes, p.k_exp + row0, kBN, &raw_full[rs]);
+        bulk_copy(dst + 2 * S::kCodes + kBN, p.v_exp + row0, kBN, &raw_full[rs]);
+      }
+      // every issued copy has landed before the CTA's shared memory goes away
+      for (int i = max(0, j - kRaw); i < j; ++i) mbar_wait(&raw_full[i % kRaw], (i / kRaw) & 1, nullptr, p.status);
+    }
+    __syncwarp();
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
     // One thread runs the whole sequence: its instructions between two MMAs are what the tensor
@@ -744,13 +768,13 @@ cudaError_t launch(const Params& p, int64_t tiles, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>(tiles), p.splits);
   cudaError_t e;
   if (p.tiles != nullptr) {
-    if ((e = ensure_smem_attr<kv8_prefill_kernel<D, true>>(Smem<D>::kBytes)) != cudaSuccess) return e;
+    if ((e = ensure_smem_attr<kv8_prefill_kernel<D, true>>(Smem<D, true>::kBytes)) != cudaSuccess) return e;
     e = launch_dependent(kv8_expand_kernel<D>, dim3(p.bt_pages, p.batch, p.hkv), kExpandThreads, 0, stream, p);
     if (e != cudaSuccess) return e;
-    e = launch_dependent(kv8_prefill_kernel<D, true>, grid, threads(true), Smem<D>::kBytes, stream, p);
+    e = launch_dependent(kv8_prefill_kernel<D, true>, grid, threads(true), Smem<D, true>::kBytes, stream, p);
   } else {
-    if ((e = ensure_smem_attr<kv8_prefill_kernel<D, false>>(Smem<D>::kBytes)) != cudaSuccess) return e;
-    e = launch_dependent(kv8_prefill_kernel<D, false>, grid, threads(false), Smem<D>::kBytes, stream, p);
+    if ((e = ensure_smem_attr<kv8_prefill_kernel<D, false>>(Smem<D, false>::kBytes)) != cudaSuccess) return e;
+    e = launch_dependent(kv8_prefill_kernel<D, false>, grid, threads(false), Smem<D, false>::kBytes, stream, p);
   }
   if (e != cudaSuccess || p.splits == 1) return e;
   const int64_t rows = static_cast<int64_t>(p.q_rows) * p.hq;
