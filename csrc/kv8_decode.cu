@@ -722,6 +722,28 @@ int kv8_decode_ctas(int sm_count, int group, int head_dim) {
                                      : (group > 8 ? Smem<64, 2>::kCtas : Smem<64, 1>::kCtas));
 }
 
+namespace {
+
+int64_t pairs_of(const Kv8AttnArgs& a) {
+  const int group = a.hq / a.hkv, heads = group > 8 ? 16 : 8;
+  return static_cast<int64_t>(a.q_rows) * a.hkv * ((group + heads - 1) / heads);
+}
+
+// Most tiles of a pair.
+int64_t most_tiles(const Kv8AttnArgs& a) {
+  if (a.window <= 0) return a.bt_pages;
+  return std::min<int64_t>(a.bt_pages, (static_cast<int64_t>(a.window) + 63) / 64 + 1 + (static_cast<int64_t>(a.sinks) + 63) / 64);
+}
+
+// CTAs per pair so that all pairs run at once, 0 where there are more pairs than CTAs.
+int widest_cluster(const Kv8AttnArgs& a) {
+  for (int c = 8; c > 0; c >>= 1)
+    if (pairs_of(a) * c <= a.ctas) return c;
+  return 0;
+}
+
+}  // namespace
+
 // CTAs of a cluster per pair, 0 for the launch over all tiles.  A cluster needs no joining launch and no
 // look-up of the other requests, but its shares follow its own request alone: taken where the pairs
 // with their clusters fit the GPU at once and no share can be long: 24 tiles at what the block table's width and
@@ -731,23 +753,21 @@ int kv8_decode_ctas(int sm_count, int group, int head_dim) {
 // 22.7 / 20.9, of 2000 31.3 / 30.3, of 3000 40.5 / 41.4; nearly a CTA for each pair, 100 slots of 3000 56.8 / 51.2, of
 // 2200 - 4500 64.7 / 64.5.
 int kv8_decode_cluster(const Kv8AttnArgs& a) {
-  const int group = a.hq / a.hkv, nt = group > 8 ? 2 : 1;
-  const int64_t pairs = static_cast<int64_t>(a.q_rows) * a.hkv * ((group + 8 * nt - 1) / (8 * nt));
-  int64_t tiles = a.bt_pages;
-  if (a.window > 0) tiles = std::min<int64_t>(tiles, (static_cast<int64_t>(a.window) + 63) / 64 + 1 + (static_cast<int64_t>(a.sinks) + 63) / 64);
-  for (int c = 8; c > 0; c >>= 1)
-    if (pairs * c <= a.ctas) return tiles <= (c == 1 && 4 * pairs >= 3 * a.ctas ? 64 : 24 * c) ? c : 0;
-  return 0;
+  const int64_t pairs = pairs_of(a), tiles = most_tiles(a);
+  const int c = widest_cluster(a);
+  return c > 0 && tiles <= (c == 1 && 4 * pairs >= 3 * a.ctas ? 64 : 24 * c) ? c : 0;
 }
 
 // Chunks of few tokens: the decode kernel reads the context once per token (mostly out of L2), the chunk
-// kernel once, but expands it.  In a graph, 32 / 4 heads of 128, microseconds by the decode / chunk kernel: one request
-// of 4 tokens on 2000 keys 7.4 / 12.0, on 32,000 24 / 28; 8 on 8000 17 / 19; 16 on 4000 17 / 18; 8 requests of 2
-// tokens on 8000 35 / 40; of 4 on 2000 17 / 20, but on 4000, without clusters, 47 / 29.
+// kernel once, but expands it.  Taken where every pair runs at once with at most 16 tiles to a CTA, and for one
+// or two tokens a request.  In a graph, 32 / 4 heads of 128, microseconds by the decode / chunk kernel: one request
+// of 4 tokens on 2000 keys 7.7 / 12.3, on 32,000 24.5 / 26.8; 8 on 8000 16.5 / 18.7, on 16,000 23.5 / 21.5; 16 on 4000
+// 16.7 / 19.1, on 16,000 36 / 24; 96 on 500 12.4 / 23.7, on 4000 48 / 31; 4 requests of 4 on 4000 16.4 / 16.7, on 8000
+// 47 / 23; 16 requests of 2 on 4000 40 / 38, on 32,000 136 / 328.
 bool kv8_few_tokens(const Kv8AttnArgs& a) {
   const int64_t rows = a.q_rows, requests = a.batch;
   if (rows > 512 || rows * a.bt_pages >= (int64_t{1} << 31)) return false;
-  return rows <= 2 * requests || kv8_decode_cluster(a) > 0 || (requests == 1 && rows <= 4);
+  return rows <= 2 * requests || most_tiles(a) <= 16 * widest_cluster(a) || (requests == 1 && rows <= 4);
 }
 
 int64_t kv8_decode_scratch_floats(int ctas, int group, int head_dim) {

@@ -11,8 +11,9 @@
 // * Keys and values enter the tensor cores as bf16 (exact: 4 significant bits times a power of two) in the
 //   swizzled shared-memory layout.  Where several row tiles see the same blocks, a launch before expands
 //   each block once into global memory as it will lie in shared memory, and one loader thread fetches it
-//   by bulk copies; the CTA then works on two query tiles.  Otherwise eight loader warps expand the
-//   blocks themselves, reading two blocks ahead, for one query tile.
+//   by bulk copies; the CTA then works on two query tiles.  Otherwise, for one query tile, one thread
+//   copies blocks of codes into a ring (four ahead) and eight loader warps expand them from there.  With
+//   the codes read by the loader warps themselves, two blocks ahead, 16 tokens on 100,000 keys took 76 us, not 57.
 // * One elected thread issues S = Q K^T and O += P V with S, P and O in tensor memory.  S has two
 //   buffers per tile, and between a PV and the S that takes its columns lie the other tile's two
 //   products, so neither the softmax nor the tensor core waits for a round trip.  P (bf16) takes
@@ -791,20 +792,31 @@ int64_t row_tiles(int64_t q_rows, int batch, int group, bool expanded) {
 }  // namespace
 
 // Bytes of the expanded tiles; 0 where the blocks are expanded in the attention kernel itself.  A launch
-// of its own costs each block a write and reads of the expanded form, but once for all row tiles.
-// One request, 32 / 4 heads of 128, microseconds with / without it: 64 new tokens (2 pairs of row tiles) on
-// 3000 keys 26 / 22, on 16,000 48 / 50, on 100,000 189 / 276; 128 tokens 31 / 28, 63 / 75, 272 / 460.
+// of its own costs each block a write and reads of the expanded form, but once for all row tiles of its
+// request: taken from four of them on, where the CTAs have enough blocks to win the launch back: 4200
+// (row tile, KV head, block) triples, 28 on each SM.  In a graph, microseconds with / without it, 32 / 4 heads of 128 (16
+// tokens a row tile): one request of 64 tokens on 16,000 keys (28 an SM) 43 / 38, on 64,000 107 / 113; 96 on 8000 (20)
+// 38 / 34, on 16,000 (40) 50 / 52; 128 on 3000 31 / 25, on 16,000 57 / 69; 1024 on themselves 31 / 28, on 1000 more 46 / 56;
+// four of 32 (two row tiles each) on 8000 50 / 42, of 64 62 / 69.
 int64_t kv8_prefill_tile_bytes(const Kv8AttnArgs& a) {
-  const int64_t step = 2 * (kRows / (a.hq / a.hkv));
+  const int64_t step = kRows / (a.hq / a.hkv);
+  int64_t seen = a.bt_pages;
+  if (a.window > 0)
+    seen = std::min<int64_t>(seen, (static_cast<int64_t>(a.window) + a.q_rows / std::max(1, a.batch)) / kPage + 2 + (static_cast<int64_t>(a.sinks) + 63) / 64);
   const int64_t bytes = static_cast<int64_t>(a.batch) * a.bt_pages * a.hkv * kPage * a.head_dim * 4;
-  if (a.q_rows < 2 * step * a.batch || bytes > (int64_t{1} << 31) || a.batch > 65535 || a.hkv > 65535) return 0;
+  if (a.q_rows < 4 * step * a.batch || a.q_rows / step * a.hkv * seen < 4200) return 0;
+  if (bytes > (int64_t{1} << 31) || a.batch > 65535 || a.hkv > 65535) return 0;
   return bytes;
 }
 
-// Splits of the key blocks: as many as keep the launch within one CTA per SM, one where the row
-// tiles alone fill the GPU.
+// Splits of the key blocks: as many as keep the launch within one CTA per SM where the requests' chunks
+// are alike, one where the row tiles alone fill the GPU.  (By the most row tiles that the lengths could make,
+// 16 chunks of 4 tokens, 32 / 4 heads of 128, on 16,000 keys took 226 us without a split, 122 with two.)
 int kv8_prefill_splits(const Kv8AttnArgs& a, int sm_count) {
-  const int64_t base = row_tiles(a.q_rows, a.batch, a.hq / a.hkv, a.tiles != nullptr) * a.hkv;
+  const int group = a.hq / a.hkv;
+  const int64_t each = static_cast<int64_t>(a.batch) * tiles_of(a.tiles != nullptr) * (kRows / group);
+  const int64_t alike = a.batch * ((a.q_rows + each - 1) / each);
+  const int64_t base = std::min(alike, row_tiles(a.q_rows, a.batch, group, a.tiles != nullptr)) * a.hkv;
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count / std::max<int64_t>(1, base), a.bt_pages)));
 }
 

@@ -489,3 +489,41 @@ def test_queries_that_are_not_finite(new):
     for t in {0, new // 2}:
         hit[t, 0] = hit[t, 5] = True
     assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(128, 8, 64), (128, 8, 128), (34, 2, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (64, 64), (150, 100), (70, 3)])
+def test_chunk_many_row_tiles(hq, hkv, d, window, sinks):
+    """Enough row tiles and blocks that the blocks are expanded by a launch of their own (a wide block table
+    counts as a long context), and few requests of few tokens, whose blocks the attention kernel expands."""
+    for q_lens, kv_lens, width in (([300, 0, 257, 290], [300, 77, 700, 291], 400), ([40, 0, 33, 2], [900, 77, 1300, 300], 60)):
+        pages = sum((n + 63) // 64 for n in kv_lens) + 2
+        cache = make_cache(pages, hkv, d, "cuda", seed=11)
+        bt = make_table(kv_lens, pages, seed=11, width=width).cuda()
+        q = torch.randn(sum(q_lens), hq * d, generator=torch.Generator().manual_seed(15)).bfloat16().cuda()
+        cu = torch.tensor([sum(q_lens[:i]) for i in range(len(q_lens) + 1)], dtype=torch.int32, device="cuda")
+        kl = torch.tensor(kv_lens, dtype=torch.int32, device="cuda")
+        out = ops.kv8_prefill_attention(q, cache, bt, cu, kl, hq, hkv, d, window=window, sinks=sinks)
+        check_attention(out, q, cache, bt, q_lens, kv_lens, hq, hkv, d, d ** -0.5, window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,new,top", [(16, 4, 3000), (3, 30, 5000), (5, 17, 2500)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_chunk_ring_of_codes(batch, new, top, d):
+    """Chunks whose blocks pass several times round both rings, split over the keys by unequal shares: more row
+    tiles than requests of equal length would make, and requests without keys before the chunk."""
+    hq, hkv = 16, 2
+    q_lens = [0 if b % 7 == 3 else 1 + (b * 5) % new for b in range(batch)]
+    q_lens[0] = 2 * new + 1
+    kv_lens = [n + (0 if b % 4 == 1 else (b * 911 + 500) % top) for b, n in enumerate(q_lens)]
+    pages = sum((n + 63) // 64 for n in kv_lens) + 2
+    cache = make_cache(pages, hkv, d, "cuda", seed=12)
+    bt = make_table(kv_lens, pages, seed=12).cuda()
+    q = torch.randn(sum(q_lens), hq * d, generator=torch.Generator().manual_seed(16)).bfloat16().cuda()
+    cu = torch.tensor([sum(q_lens[:i]) for i in range(len(q_lens) + 1)], dtype=torch.int32, device="cuda")
+    kl = torch.tensor(kv_lens, dtype=torch.int32, device="cuda")
+    for window, sinks in ((0, 0), (700, 5)):
+        out = ops.kv8_prefill_attention(q, cache, bt, cu, kl, hq, hkv, d, window=window, sinks=sinks)
+        check_attention(out, q, cache, bt, q_lens, kv_lens, hq, hkv, d, d ** -0.5, window, sinks)
