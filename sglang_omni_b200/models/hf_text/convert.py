@@ -11,8 +11,8 @@ Covered configuration fields: GQA heads and head_dim, q / k / v biases (Qwen2; L
 ``attention_bias``), per-head q / k RMSNorm (Qwen3), RoPE theta with linear or Llama-3 frequency
 scaling, tied embeddings, softmax top-k routed experts with optional top-k renormalisation and
 dense ``mlp_only_layers`` / ``decoder_sparse_step`` layers (Qwen3-MoE); with the 8-bit KV pool
-(``kv_format="e4m3"``) sliding-window attention (Mistral v0.1 style, Qwen2 ``use_sliding_window``
-from ``max_window_layers`` on, ``layer_types``).  Refused with a message: sliding windows with the
+(``kv_format="e4m3"``) sliding-window attention (Mistral v0.1 style and Qwen3-MoE in every layer, Qwen2 and
+Qwen3 by ``layer_types`` or from ``max_window_layers`` on).  Refused with a message: sliding windows with the
 native KV pool, MLP biases, other RoPE scalings."""
 from __future__ import annotations
 
@@ -27,6 +27,9 @@ from ..weight_loader import load_by_prefix, load_decoder_from_hf
 
 SUPPORTED_ARCHITECTURES = ("LlamaForCausalLM", "MistralForCausalLM", "Qwen2ForCausalLM", "Qwen3ForCausalLM",
                            "Qwen3MoeForCausalLM")
+# architectures whose transformers model has a sliding window, and their model types
+_WINDOW_KINDS = {"MistralForCausalLM": "mistral", "Qwen2ForCausalLM": "qwen2", "Qwen3ForCausalLM": "qwen3",
+                 "Qwen3MoeForCausalLM": "qwen3_moe"}
 
 
 def _get(c, name, default=None):
@@ -42,6 +45,35 @@ def _rope(c) -> tuple[float, dict | None]:
     return float(theta), (dict(scaling) if scaling else None)
 
 
+def _window(c, arch: str, layers: int, max_position: int, kv_format: str) -> dict:
+    """``sliding_window`` / ``window_layers`` of a checkpoint, by transformers' rule for its architecture:
+    Mistral and Qwen3-MoE have the window in every layer, Qwen2 and Qwen3 in the layers that ``layer_types``
+    names, or without it from ``max_window_layers`` (28) on; the Qwen models only with ``use_sliding_window``.
+    A window in an architecture that has none there is refused, as is every window with the native KV pool."""
+    win = _get(c, "sliding_window")
+    if kv_format == "native":
+        if win and _get(c, "use_sliding_window", arch != "Qwen2ForCausalLM") and int(win) < max_position:
+            raise NotImplementedError(f"{arch}: sliding-window attention ({win}) is not supported by the paged engine's "
+                                      "native KV pool; kv_format='e4m3' serves it")
+        return {}
+    kind = _WINDOW_KINDS.get(arch) or str(_get(c, "model_type") or "")
+    known = kind in _WINDOW_KINDS.values()
+    if known and isinstance(c, dict) and "sliding_window" not in c:
+        win = 4096                            # transformers' default of a field that the file does not have
+    uses = _get(c, "use_sliding_window", not kind.startswith("qwen")) or kind == "mistral"
+    if not win or not uses or int(win) >= max_position:
+        return {}
+    kinds = _get(c, "layer_types") if kind in ("qwen2", "qwen3") else None
+    if not known or (kinds and (len(kinds) != layers or not set(kinds) <= {"sliding_attention", "full_attention"})):
+        raise NotImplementedError(f"{arch or kind}: a sliding window ({win}) with layer_types {kinds} is not supported")
+    if kinds:
+        windowed = tuple(i for i, k in enumerate(kinds) if k == "sliding_attention")
+    else:
+        first = int(_get(c, "max_window_layers", 28)) if kind in ("qwen2", "qwen3") else 0
+        windowed = tuple(range(first, layers))
+    return dict(sliding_window=int(win), window_layers=windowed)
+
+
 def decoder_config_from_hf(c: Any, dtype: torch.dtype = torch.bfloat16, max_position: int | None = None,
                            kv_format: str = "native") -> DecoderConfig:
     """``c``: a transformers ``PretrainedConfig`` or its ``config.json`` dict."""
@@ -52,18 +84,7 @@ def decoder_config_from_hf(c: Any, dtype: torch.dtype = torch.bfloat16, max_posi
     heads = int(_get(c, "num_attention_heads"))
     hidden = int(_get(c, "hidden_size"))
     layers = int(_get(c, "num_hidden_layers"))
-    win = _get(c, "sliding_window")
-    if win and (_get(c, "use_sliding_window", arch != "Qwen2ForCausalLM") and int(win) < int(
-            max_position or _get(c, "max_position_embeddings") or 0)):
-        if kv_format == "native":
-            raise NotImplementedError(f"{arch}: sliding-window attention ({win}) is not supported by the paged engine's "
-                                      "native KV pool; kv_format='e4m3' serves it")
-        kinds = list(_get(c, "layer_types") or [])
-        first = int(_get(c, "max_window_layers") or 0) if arch.startswith("Qwen") else 0
-        window = dict(sliding_window=int(win), window_layers=tuple(
-            i for i in range(layers) if (kinds[i] == "sliding_attention" if len(kinds) == layers else i >= first)))
-    else:
-        window = {}
+    window = _window(c, arch, layers, int(max_position or _get(c, "max_position_embeddings") or 0), kv_format)
     if _get(c, "mlp_bias", False):
         raise NotImplementedError(f"{arch}: MLP biases are not supported")
     theta, scaling = _rope(c)
