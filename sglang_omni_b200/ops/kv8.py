@@ -95,6 +95,7 @@ def kv8_attention_ref(q, cache: KV8Cache, block_table, q_lens, kv_lens, num_head
     out = torch.zeros(q.shape[0], num_heads, head_dim, dtype=dt, device=q.device)
     g, at = num_heads // num_kv_heads, 0
     for b, (a, n) in enumerate(zip(q_lens, kv_lens)):
+        n = min(n, block_table.shape[1] * PAGE)     # a request sees at most the keys that its row can name
         if a > 0 and n > 0:
             j = torch.arange(n, device=q.device)
             pages = block_table[b, j // PAGE].long()
