@@ -252,10 +252,31 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
   return out;
 }
 
+// The form that kv8_attention takes for a chunk batch of these sizes: "decode" (every token a request of its
+// own), "expanded" (key blocks expanded by a launch before) or "in place" (by the attention kernel itself).
+std::string kv8_chunk_form(int64_t q_rows, int64_t requests, int64_t table_pages, int64_t hq, int64_t hkv,
+                           int64_t head_dim, int64_t window, int64_t sinks) {
+  TORCH_CHECK(q_rows >= 0 && requests >= 1 && table_pages >= 0 && hkv >= 1 && hq >= hkv && hq / hkv <= 128 && window >= 0 && sinks >= 0,
+              "kv8_chunk_form: sizes out of range");
+  omni::Kv8AttnArgs a{};
+  a.q_rows = static_cast<int>(q_rows);
+  a.batch = static_cast<int>(requests);
+  a.bt_pages = static_cast<int>(table_pages);
+  a.hq = static_cast<int>(hq);
+  a.hkv = static_cast<int>(hkv);
+  a.head_dim = static_cast<int>(head_dim);
+  a.window = static_cast<int>(window);
+  a.sinks = static_cast<int>(sinks);
+  a.ctas = omni::kv8_decode_ctas(at::cuda::getCurrentDeviceProperties()->multiProcessorCount, static_cast<int>(hq / hkv), a.head_dim);
+  if (omni::kv8_few_tokens(a)) return "decode";
+  return omni::kv8_prefill_tile_bytes(a) > 0 ? "expanded" : "in place";
+}
+
 }  // namespace
 
 void bind_kv8(pybind11::module_& m) {
   m.def("kv8_store", &kv8_store, "QK RMSNorm + (M-)RoPE + quantised store into the 8-bit paged KV cache");
   m.def("kv8_read", &kv8_read, "rows of the 8-bit paged KV cache by slot, as bf16");
   m.def("kv8_attention", &kv8_attention, "paged GQA attention over the 8-bit KV cache (decode: cu_q None)");
+  m.def("kv8_chunk_form", &kv8_chunk_form, "the form that kv8_attention takes for a chunk batch of these sizes");
 }

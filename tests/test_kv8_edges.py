@@ -3,7 +3,6 @@ import pytest
 import torch
 
 from sglang_omni_b200 import ops
-from sglang_omni_b200.ops import kv8 as K
 from test_kv8 import check_attention, make_cache, make_table
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
