@@ -5,6 +5,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+
 #include "omni_kernels.h"
 
 namespace {
@@ -95,6 +97,9 @@ torch::Tensor kv8_store(const torch::Tensor& qkv, const torch::Tensor& k, const 
     TORCH_CHECK((positions->dim() == 1 || positions->dim() == 2) && (a.pos_rows == 1 || a.pos_rows == 3) &&
                     positions->numel() == a.pos_rows * T,
                 "positions must be [T] or [3, T]");
+    TORCH_CHECK(section.empty() || (section.size() == 3 && section[0] >= 0 && section[1] >= 0 && section[2] >= 0),
+                "mrope_section must be empty or three sizes");
+    if (section.empty()) a.pos_rows = 1;   // without sections every pair follows the first row
     for (const auto* t : {&*cos_tab, &*sin_tab}) {
       check_on(*t, k, "cos_tab / sin_tab");
       TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(1) == rot_dim / 2 && t->is_contiguous() &&
@@ -127,7 +132,7 @@ torch::Tensor kv8_store(const torch::Tensor& qkv, const torch::Tensor& k, const 
   a.q_norm = q_norm.has_value() ? q_norm->data_ptr() : nullptr;
   a.k_norm = k_norm.has_value() ? k_norm->data_ptr() : nullptr;
   a.eps = static_cast<float>(eps);
-  for (int i = 0; i < 3; ++i) a.section[i] = i < static_cast<int>(section.size()) ? static_cast<int>(section[i]) : 0;
+  for (size_t i = 0; i < section.size() && i < 3; ++i) a.section[i] = static_cast<int>(std::min<int64_t>(section[i], head_dim));
   a.interleaved = interleaved ? 1 : 0;
   a.rot_dim = static_cast<int>(rot_dim);
   a.neox = neox ? 1 : 0;

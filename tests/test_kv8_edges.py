@@ -33,3 +33,21 @@ def test_lengths_beyond_the_block_table(device, width):
         return
     check_attention(out, q[:1], cache, bt, [1], [n], hq, hkv, d, d ** -0.5, 0, 0)
     check_attention(chunk, q, cache, bt, [3], [n], hq, hkv, d, d ** -0.5, 0, 0)
+
+
+@pytest.mark.gpu
+def test_three_position_rows_without_sections():
+    """Without sections every pair follows the first position row, whatever the kind of sections would be."""
+    hq, hkv, d, n = 2, 1, 64, 9
+    qkv = torch.randn(n, (hq + 2 * hkv) * d, generator=torch.Generator().manual_seed(2)).bfloat16()
+    cos, sin = (torch.randn(2, 40, d // 2, generator=torch.Generator().manual_seed(3))).unbind(0)
+    pos = torch.stack([torch.arange(n), torch.arange(n) + 11, torch.arange(n) + 23]).int()
+    one = ops.KV8Cache.zeros(2, hkv, d, "cuda")
+    want = ops.kv8_store(qkv.cuda(), one, i32("cuda", *range(n)), hq, hkv, d, pos[0].contiguous().cuda(), cos.cuda(), sin.cuda())
+    for interleaved in (True, False):
+        cache = ops.KV8Cache.zeros(2, hkv, d, "cuda")
+        q = ops.kv8_store(qkv.cuda(), cache, i32("cuda", *range(n)), hq, hkv, d, pos.cuda(), cos.cuda(), sin.cuda(), interleaved=interleaved)
+        assert torch.equal(q, want) and torch.equal(cache.k.view(torch.uint8), one.k.view(torch.uint8))
+    for section in ([8, 24], [8, 8, 8, 8], [16, 24, -8]):
+        with pytest.raises(RuntimeError):
+            ops.kv8_store(qkv.cuda(), one, i32("cuda", *range(n)), hq, hkv, d, pos.cuda(), cos.cuda(), sin.cuda(), mrope_section=section)
