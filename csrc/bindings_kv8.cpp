@@ -222,7 +222,8 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
   a.hkv = static_cast<int>(hkv);
   a.head_dim = static_cast<int>(head_dim);
   a.scale = static_cast<float>(scale);
-  a.window = static_cast<int>(window);
+  // a window that no context exceeds is none (and the kernels' 32-bit positions minus it stay in range)
+  a.window = window < a.bt_pages * int64_t{64} ? static_cast<int>(window) : 0;
   a.sinks = static_cast<int>(sinks);
   a.out = out.data_ptr();
   a.out_stride = out.stride(0);
@@ -270,7 +271,7 @@ std::string kv8_chunk_form(int64_t q_rows, int64_t requests, int64_t table_pages
   a.hq = static_cast<int>(hq);
   a.hkv = static_cast<int>(hkv);
   a.head_dim = static_cast<int>(head_dim);
-  a.window = static_cast<int>(window);
+  a.window = window < table_pages * 64 ? static_cast<int>(window) : 0;
   a.sinks = static_cast<int>(sinks);
   a.ctas = omni::kv8_decode_ctas(at::cuda::getCurrentDeviceProperties()->multiProcessorCount, static_cast<int>(hq / hkv), a.head_dim);
   if (omni::kv8_few_tokens(a)) return "decode";

@@ -51,3 +51,20 @@ def test_three_position_rows_without_sections():
     for section in ([8, 24], [8, 8, 8, 8], [16, 24, -8]):
         with pytest.raises(RuntimeError):
             ops.kv8_store(qkv.cuda(), one, i32("cuda", *range(n)), hq, hkv, d, pos.cuda(), cos.cuda(), sin.cuda(), mrope_section=section)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 64, 2 ** 30])
+@pytest.mark.parametrize("new,kv,width", [(100, 90, 4), (300, 130, 400), (600, 500, 400), (3, 2, 1)])
+def test_windows_beyond_every_context(window, new, kv, width):
+    """A window longer than the block table can name sees all keys, in chunks longer than their context too
+    (whose first queries see none)."""
+    hq, hkv, d = 32, 4, 64
+    pages = (kv + 63) // 64
+    cache = make_cache(pages + 2, hkv, d, "cuda", seed=4)
+    bt = make_table([kv], pages + 2, seed=4, width=width).cuda()
+    q = queries(new, hq * d, 4, "cuda")
+    out = ops.kv8_prefill_attention(q, cache, bt, i32("cuda", 0, new), i32("cuda", kv), hq, hkv, d, window=window, sinks=2)
+    check_attention(out, q, cache, bt, [new], [kv], hq, hkv, d, d ** -0.5, 0, 0)
+    last = ops.kv8_decode_attention(q[-1:], cache, bt, i32("cuda", kv), hq, hkv, d, window=window, sinks=2)
+    check_attention(last, q[-1:], cache, bt, [1], [kv], hq, hkv, d, d ** -0.5, 0, 0)
