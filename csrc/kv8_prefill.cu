@@ -607,21 +607,26 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
     const int tok = tok0 + t * p.tpt + in;
     const int head = h * p.G + (r - in * p.G);
     const bool row_ok = t < tiles && in < p.tpt && tok < q_len;
-    if (t < tiles && nb > 0) {
-      const __nv_bfloat16* src = p.q + static_cast<int64_t>(q_begin + (row_ok ? tok : 0)) * p.q_stride + static_cast<int64_t>(head) * D;
-      uint8_t* dst = smem + S::kQ + t * S::kQBytes + r * 128;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        const uint4 x = row_ok ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * kRegionQ + (((c & 7) ^ (r & 7)) << 4)) = x;
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&q_full[t]);
-    }
     // a row without a query keeps every key: its results are not stored
     const int qpos = row_ok ? past + tok : 0x3fffffff;
     const int low = row_ok && p.window > 0 ? qpos - p.window : -1;   // keys <= low are seen only below `sinks`
     float m_run = -INFINITY, l_run = 0.f;
+    if (t < tiles && nb > 0) {
+      const __nv_bfloat16* src = p.q + static_cast<int64_t>(q_begin + (row_ok ? tok : 0)) * p.q_stride + static_cast<int64_t>(head) * D;
+      uint8_t* dst = smem + S::kQ + t * S::kQBytes + r * 128;
+      uint32_t top = 0;                               // largest magnitudes of the even and of the odd elements
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 x = row_ok ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * kRegionQ + (((c & 7) ^ (r & 7)) << 4)) = x;
+        top = __vmaxu2(__vmaxu2(top, x.x & 0x7fff7fffu), __vmaxu2(x.y & 0x7fff7fffu, __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&q_full[t]);
+      // An infinite query whose scores are all -inf would look like one that sees nothing: its sum is NaN from
+      // the start, unless it does see nothing.
+      if (((top & 0xffffu) >= 0x7f80u || top >= 0x7f800000u) && qpos >= 0) l_run = NAN;
+    }
     bool ok = true;
     const int n = t < tiles ? nb : 0;
     for (int j = 0; j < n && ok; ++j) {

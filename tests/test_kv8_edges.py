@@ -68,3 +68,20 @@ def test_windows_beyond_every_context(window, new, kv, width):
     check_attention(out, q, cache, bt, [new], [kv], hq, hkv, d, d ** -0.5, 0, 0)
     last = ops.kv8_decode_attention(q[-1:], cache, bt, i32("cuda", kv), hq, hkv, d, window=window, sinks=2)
     check_attention(last, q[-1:], cache, bt, [1], [kv], hq, hkv, d, d ** -0.5, 0, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,past,width", [(1, 0, 1), (40, 0, 1), (40, 3000, 60), (300, 0, 200)])
+@pytest.mark.parametrize("window", [0, 1])
+def test_infinite_queries_that_see_few_keys(new, past, width, window):
+    """A query with an infinity whose scores are all negative infinity has no softmax: NaN, not zeros."""
+    hq, hkv, d = 16, 2, 128
+    n = new + past
+    cache = make_cache((n + 63) // 64 + 2, hkv, d, "cuda", seed=5)
+    bt = make_table([n], (n + 63) // 64 + 2, seed=5, width=max(width, (n + 63) // 64)).cuda()
+    q = queries(new, hq * d, 5, "cuda")
+    for h in range(0, hq, 3):
+        q[:, h * d + 5 * h] = float("inf") if h % 2 else float("-inf")
+    out = ops.kv8_prefill_attention(q, cache, bt, i32("cuda", 0, new), i32("cuda", n), hq, hkv, d, window=window)
+    assert torch.isnan(out.view(new, hq, d)[:, ::3]).all()
+    check_attention(out, q, cache, bt, [new], [n], hq, hkv, d, d ** -0.5, window, 0)
