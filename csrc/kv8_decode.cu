@@ -259,6 +259,10 @@ __device__ __forceinline__ float2 ld_dsmem_f2(uint32_t addr) {
   return v;
 }
 
+// A row's exponent clamped into the format, from its lowest: min(max(e - kExpMin, 0), kExpMax - kExpMin), one
+// instruction.  (64 slots of about 1150 keys: clamped so 20.7 us, in two instructions 20.9, not at all 20.5.)
+__device__ __forceinline__ int clamped(int e) { return __viaddmin_s32_relu(e, -kExpMin, kExpMax - kExpMin); }
+
 // Byte offset of 16-byte chunk c of row r in a swizzled tile (128-byte swizzle for 128-byte rows,
 // 64-byte swizzle for 64-byte rows).
 template <int D>
@@ -455,9 +459,10 @@ __global__ void __launch_bounds__(kThreads, Smem<D, NT>::kCtas)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int ke = ex[16 * q + 8 * u], ve = ex[kPage + 16 * q + 8 * u];
-          const float kf = __int_as_float(0x3f800000 + (ke << 23));
-          const float vf = min(ke, ve) == kExpBad ? __int_as_float(0x7fc00000) : __int_as_float(0x4b400000 + ve) - 12582912.f;
-          vi[q][u] = __int_as_float(0x3f800000 - (ve << 23));
+          const int kc = clamped(ke), vc = clamped(ve);
+          const float kf = __int_as_float(((127 + kExpMin) << 23) + (kc << 23));
+          const float vf = min(ke, ve) == kExpBad ? __int_as_float(0x7fc00000) : __int_as_float(0x4b400000 + vc) - (12582912.f - kExpMin);
+          vi[q][u] = __int_as_float(((127 - kExpMin) << 23) - (vc << 23));
           const bool in = !kEdge || seen(key0 + row0 + 16 * q + 8 * u + g);
           if (!in) vi[q][u] = 0.f;
 #pragma unroll

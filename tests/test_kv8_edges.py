@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from sglang_omni_b200 import ops
-from test_kv8 import check_attention, make_cache, make_table
+from test_kv8 import check_attention, make_cache, make_table, to
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -85,3 +85,31 @@ def test_infinite_queries_that_see_few_keys(new, past, width, window):
     out = ops.kv8_prefill_attention(q, cache, bt, i32("cuda", 0, new), i32("cuda", n), hq, hkv, d, window=window)
     assert torch.isnan(out.view(new, hq, d)[:, ::3]).all()
     check_attention(out, q, cache, bt, [new], [n], hq, hkv, d, d ** -0.5, window, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,width", [(1, 3), (40, 3), (300, 400)])
+def test_exponents_outside_the_format(new, width):
+    """Exponents that no write leaves (a cache made by hand) count as the nearest of the format, in every operator."""
+    hq, hkv, d, n = 16, 2, 128, 190 if new < 300 else 330
+    pages = (n + 63) // 64 + 1
+    for case in range(2):
+        cache = make_cache(pages, hkv, d, "cpu", seed=6)
+        bt = make_table([n], pages, seed=6, width=max(width, pages))
+        at = lambda j: (bt[0, j // 64], slice(None), j % 64)  # noqa: E731
+        if case == 0:
+            cache.k_exp[at(0)], cache.v_exp[at(0)] = -127, -61
+            cache.k_exp[at(70)], cache.v_exp[at(70)] = -90, -127
+            cache.k.view(torch.uint8)[at(100)], cache.k_exp[at(100)] = 0, 127        # zero keys: the score stays 0
+            cache.k.view(torch.uint8)[at(101)], cache.k_exp[at(101)] = 0, 61
+        else:
+            cache.v_exp[at(1)], cache.v_exp[at(2)], cache.v_exp[at(90)] = 61, 127, 100
+        dev = to(cache, "cuda")
+        q = queries(new, hq * d, 6, "cuda")
+        out = ops.kv8_prefill_attention(q, dev, bt.cuda(), i32("cuda", 0, new), i32("cuda", n), hq, hkv, d)
+        check_attention(out, q, cache, bt, [new], [n], hq, hkv, d, d ** -0.5, 0, 0)
+        last = ops.kv8_decode_attention(q[:1], dev, bt.cuda(), i32("cuda", n), hq, hkv, d)
+        check_attention(last, q[:1], cache, bt, [1], [n], hq, hkv, d, d ** -0.5, 0, 0)
+        slots = torch.tensor([int(bt[0, j // 64]) * 64 + j % 64 for j in range(n)], dtype=torch.int32)
+        for a, b in zip(ops.kv8_read(dev, slots.cuda()), ops.kv8_read(cache, slots)):
+            assert torch.equal(a.cpu(), b)
