@@ -13,7 +13,7 @@
 //   each block once into global memory as it will lie in shared memory, and one loader thread fetches it
 //   by bulk copies; the CTA then works on two query tiles.  Otherwise, for one query tile, one thread
 //   copies blocks of codes into a ring (four ahead) and eight loader warps expand them from there.  With
-//   the codes read by the loader warps themselves, two blocks ahead, 16 tokens on 100,000 keys took 76 us, not 57.
+//   the codes read by the loader warps themselves, two blocks ahead, 16 tokens on 100,000 keys took 76 us, not 59.
 // * One elected thread issues S = Q K^T and O += P V with S, P and O in tensor memory.  S has two
 //   buffers per tile, and between a PV and the S that takes its columns lie the other tile's two
 //   products, so neither the softmax nor the tensor core waits for a round trip.  P (bf16) takes
@@ -491,14 +491,17 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
         const int8_t* e = reinterpret_cast<const int8_t*>(k + 2 * S::kCodes);
         Part<D, TH> part;
         part.fetch(k, k + S::kCodes, e, e + kBN, tid);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&raw_empty[rs]);
         if (j >= kStages && !warp_wait(&kv_empty[stage], phase, abort_flag, p.status, 41)) break;
         uint8_t* dk = smem + S::kKV + stage * 2 * S::kKBytes;
         part.store(dk, dk + S::kKBytes, kv_len - block_of(j) * kPage, tid);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[stage]);
+        if (lane == 0) {
+          mbar_arrive(&kv_full[stage]);
+          // Only now: the codes have been used.  Released right after their loads, a slot could be filled again
+          // while a load was still to come, and rows of the block four ahead took their places.
+          mbar_arrive(&raw_empty[rs]);
+        }
         if (++stage == kStages) stage = 0, phase ^= 1;
       }
     }

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from sglang_omni_b200 import ops
+from sglang_omni_b200.ops._ext import ext
 from test_kv8 import check_attention, make_cache, make_table, to
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -113,3 +114,29 @@ def test_exponents_outside_the_format(new, width):
         slots = torch.tensor([int(bt[0, j // 64]) * 64 + j % 64 for j in range(n)], dtype=torch.int32)
         for a, b in zip(ops.kv8_read(dev, slots.cuda()), ops.kv8_read(cache, slots)):
             assert torch.equal(a.cpu(), b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,new,past,width,d", [
+    ("in place", 900, 700, 25, 128), ("in place", 700, 900, 25, 128), ("in place", 600, 700, 21, 64), ("in place", 130, 3000, 60, 128),
+    ("expanded", 900, 700, 400, 128), ("expanded", 900, 700, 400, 64), ("decode", 8, 900, 20, 128)])
+def test_chunk_among_other_launches(name, new, past, width, d):
+    """The same bits whatever runs around it: stores before and behind it, and itself, launched back to back."""
+    hq, hkv, n = 16, 4, new + past
+    pages = (n + 63) // 64
+    cache, other = make_cache(pages + 2, hkv, d, "cuda", seed=9), ops.KV8Cache.zeros(20, hkv, d, "cuda")
+    bt = make_table([n], pages + 2, seed=9, width=width).cuda()
+    assert ext().kv8_chunk_form(new, 1, width, hq, hkv, d, 0, 0) == name
+    rows = torch.randn(900, (hq + 2 * hkv) * d, generator=torch.Generator().manual_seed(10)).bfloat16().cuda()
+    slots = torch.arange(900, dtype=torch.int32, device="cuda")
+    cu, kl = i32("cuda", 0, new), i32("cuda", n)
+    for size in (0.02, 3.0):                       # flat and sharp softmaxes
+        q = (size * torch.randn(new, hq * d, generator=torch.Generator().manual_seed(11))).bfloat16().cuda()
+        first = ops.kv8_prefill_attention(q, cache, bt, cu, kl, hq, hkv, d)
+        check_attention(first, q, cache, bt, [new], [n], hq, hkv, d, d ** -0.5, 0, 0)
+        for _ in range(8):
+            outs = []
+            for _ in range(8):
+                ops.kv8_store(rows, other, slots, hq, hkv, d)
+                outs.append(ops.kv8_prefill_attention(q, cache, bt, cu, kl, hq, hkv, d))
+            assert all(torch.equal(o, first) for o in outs)
