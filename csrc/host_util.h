@@ -28,7 +28,9 @@ cudaError_t ensure_smem_attr(int bytes) {
 }
 
 // A launch that may start while the one before it on the stream still runs (programmatic dependent
-// launch): every thread of its kernel calls grid_dep_wait() before it reads memory or exits.
+// launch): every thread of its kernel calls grid_dep_wait() before it exits, and before it reads or writes
+// memory.  What the kernels before the one before it wrote may be read earlier only if that one calls
+// grid_dep_launch() behind its own grid_dep_wait() (kv8_decode_kernel and its join).
 template <class... Args>
 cudaError_t launch_dependent_cluster(void (*kernel)(Args...), dim3 grid, int block, int smem, int cluster,
                                      cudaStream_t stream, const Args&... args) {

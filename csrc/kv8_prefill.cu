@@ -377,7 +377,6 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   grid_dep_wait();
-  grid_dep_launch();
 
   // Row tile and KV head of this CTA.  The grid hands CTAs out in order, and the last to start should be
   // short: requests by falling context (up to 32 of them; by position in the batch beyond), each
@@ -458,6 +457,7 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_dep_launch();   // with tensor memory in hand: a dependent may allocate its own before it waits for this grid
   const uint32_t tmem = *tmem_slot;
   auto s_col = [](int t, int b) -> uint32_t { return static_cast<uint32_t>(t * 2 + b) * 64u; };
   auto o_col = [](int t) -> uint32_t { return 256u + static_cast<uint32_t>(t) * D; };

@@ -127,7 +127,7 @@ def test_chunk_among_other_launches(name, new, past, width, d):
     cache, other = make_cache(pages + 2, hkv, d, "cuda", seed=9), ops.KV8Cache.zeros(20, hkv, d, "cuda")
     bt = make_table([n], pages + 2, seed=9, width=width).cuda()
     assert ext().kv8_chunk_form(new, 1, width, hq, hkv, d, 0, 0) == name
-    rows = torch.randn(900, (hq + 2 * hkv) * d, generator=torch.Generator().manual_seed(10)).bfloat16().cuda()
+    rows = torch.randn(900, (8 + 2 * hkv) * d, generator=torch.Generator().manual_seed(10)).bfloat16().cuda()
     slots = torch.arange(900, dtype=torch.int32, device="cuda")
     cu, kl = i32("cuda", 0, new), i32("cuda", n)
     for size in (0.02, 3.0):                       # flat and sharp softmaxes
@@ -137,6 +137,41 @@ def test_chunk_among_other_launches(name, new, past, width, d):
         for _ in range(8):
             outs = []
             for _ in range(8):
-                ops.kv8_store(rows, other, slots, hq, hkv, d)
+                ops.kv8_store(rows, other, slots, 8, hkv, d)
                 outs.append(ops.kv8_prefill_attention(q, cache, bt, cu, kl, hq, hkv, d))
             assert all(torch.equal(o, first) for o in outs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [60, 900])
+@pytest.mark.parametrize("d", [64, 128])
+def test_dependent_launches_behind_a_chunk(new, d):
+    """A GEMM and the next layer's store and attention, launched while the chunk attention runs, give what they
+    give one by one."""
+    hq, hkv, n = 16, 2, new + 700
+    caches = [make_cache((n + 63) // 64 + 2, hkv, d, "cuda", seed=s) for s in (7, 8)]
+    bt = make_table([n], (n + 63) // 64 + 2, seed=7, width=(n + 63) // 64).cuda()
+    q = queries(new, hq * d, 7, "cuda")
+    g = torch.Generator().manual_seed(8)
+    w = (torch.randn((hq + 2 * hkv) * d, hq * d, generator=g) * d ** -0.5 / 4).bfloat16().cuda()
+    slots = torch.tensor([int(bt[0, j // 64]) * 64 + j % 64 for j in range(n - new, n)], dtype=torch.int32, device="cuda")
+    cu, kl = i32("cuda", 0, new), i32("cuda", n)
+
+    def layers(wait):
+        own = [to(c, "cpu") for c in caches]
+        own = [to(c, "cuda") for c in own] * 3
+        x, outs = q, []
+        for c in own:
+            x = ops.kv8_prefill_attention(x, c, bt, cu, kl, hq, hkv, d)
+            wait()
+            y = ops.linear(x, w)
+            wait()
+            x = ops.kv8_store(y, c, slots, hq, hkv, d)
+            wait()
+            outs += [y, x]
+        return outs
+
+    want = layers(torch.cuda.synchronize)
+    for _ in range(3):
+        for a, b in zip(layers(lambda: None), want):
+            assert torch.equal(a, b)
