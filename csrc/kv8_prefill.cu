@@ -107,6 +107,7 @@ struct Params {
   float* part_o;                           // [splits][q_rows * hq][D]
   float2* part_ml;                         // [splits][q_rows * hq]
   uint8_t* tiles;                          // expanded K / V tiles, or nullptr
+  int slots, slots_by_tok;                 // tiles of a request begin at req * slots (+ its first query row / 64)
   int* status;
 };
 
@@ -329,19 +330,36 @@ struct Blocks {
     count = end > 0 ? sink_blocks + ((end + 63) >> 6) - first : 0;
   }
   __device__ int at(int j) const { return j < sink_blocks ? j : first + j - sink_blocks; }
+  __device__ int of(int page) const { return page < sink_blocks ? page : sink_blocks + page - first; }   // at()'s inverse
+};
+
+// A request's new tokens (rows q_begin .. q_begin + q_len - 1 of q; cu_q never names rows past q) and its keys.
+struct Chunk {
+  int q_begin, q_len, kv_len;
+  int past;                                                     // keys before the chunk's first query
+  __device__ Chunk(const Params& p, int req) {
+    q_begin = min(max(0, p.cu_q[req]), p.q_rows);
+    q_len = min(p.cu_q[req + 1], p.q_rows) - q_begin;
+    kv_len = max(0, min(p.kv_lens[req], p.bt_pages * kPage));
+    past = kv_len - (p.cu_q[req + 1] - q_begin);
+  }
+  // Its first tile of p.tiles.  With a window a request of n tokens sees at most slots + n / 64 blocks, and
+  // req * slots + q_begin / 64 leaves room for them without a look at the others' lengths.
+  __device__ int64_t first_tile(const Params& p, int req) const {
+    return static_cast<int64_t>(req) * p.slots + (p.slots_by_tok ? q_begin >> 6 : 0);
+  }
 };
 
 // Expands every block that a request's new tokens see, once, into `tiles` (K tile, V tile of each
-// [request][page][KV head], as they will lie in shared memory).
+// [request][block][KV head], as they will lie in shared memory).
 template <int D>
 __global__ void __launch_bounds__(kExpandThreads) kv8_expand_kernel(const Params p) {
   grid_dep_wait();
   grid_dep_launch();
   const int req = blockIdx.y, h = blockIdx.z;
-  const int n = p.cu_q[req + 1] - p.cu_q[req];
-  const int kv_len = max(0, min(p.kv_lens[req], p.bt_pages * kPage));
-  if (n <= 0) return;
-  const Blocks bl(p, kv_len, kv_len - n, n);
+  const Chunk c(p, req);
+  if (c.q_len <= 0) return;
+  const Blocks bl(p, c.kv_len, c.past, c.q_len);
   if (static_cast<int>(blockIdx.x) >= bl.count) return;
   const int i = bl.at(blockIdx.x);
   const int page = checked_page(p.block_table[static_cast<int64_t>(req) * p.bt_stride + i], p.num_pages);
@@ -349,8 +367,8 @@ __global__ void __launch_bounds__(kExpandThreads) kv8_expand_kernel(const Params
   const int64_t row0 = (static_cast<int64_t>(page) * p.hkv + h) * kPage;
   part.fetch(p.k + row0 * D, p.v + row0 * D, p.k_exp + row0, p.v_exp + row0, threadIdx.x);
   constexpr int kTile = Smem<D, true>::kKBytes;
-  uint8_t* dst = p.tiles + ((static_cast<int64_t>(req) * p.bt_pages + i) * p.hkv + h) * (2 * kTile);
-  part.store(dst, dst + kTile, kv_len - i * kPage, threadIdx.x);
+  uint8_t* dst = p.tiles + ((c.first_tile(p, req) + blockIdx.x) * p.hkv + h) * (2 * kTile);
+  part.store(dst, dst + kTile, c.kv_len - i * kPage, threadIdx.x);
 }
 
 // kExpanded: the K / V tiles come ready from kv8_expand_kernel by bulk copies.
@@ -418,10 +436,8 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
     }
     if (req < 0) return;
   }
-  const int q_begin = max(0, p.cu_q[req]);
-  const int q_len = min(p.cu_q[req + 1], p.q_rows) - q_begin;   // cu_q never names rows past q
-  const int kv_len = max(0, min(p.kv_lens[req], p.bt_pages * kPage));
-  const int past = kv_len - (p.cu_q[req + 1] - q_begin);        // keys before the chunk's first query
+  const Chunk chunk(p, req);
+  const int q_begin = chunk.q_begin, q_len = chunk.q_len, kv_len = chunk.kv_len, past = chunk.past;
   const int tiles = kTiles == 2 && q_len - tok0 > p.tpt ? 2 : 1;
   const Blocks bl(p, kv_len, past + tok0, min(q_len - tok0, kTiles * p.tpt));
   const int j0 = static_cast<int>(static_cast<int64_t>(bl.count) * z / p.splits);
@@ -468,12 +484,13 @@ __global__ void __launch_bounds__(threads(kExpanded), 1) kv8_prefill_kernel(cons
     uint32_t phase = 1;                     // the first round finds the ring empty
     if constexpr (kExpanded) {
       if (elect_one()) {
-        const uint8_t* src = p.tiles + (static_cast<int64_t>(req) * p.bt_pages * p.hkv + h) * (2 * S::kKBytes);
+        const Blocks all(p, kv_len, past, q_len);               // as the expansion numbered them
+        const uint8_t* src = p.tiles + (chunk.first_tile(p, req) * p.hkv + h) * (2 * S::kKBytes);
         int j = 0;
         for (; j < nb; ++j) {
           if (j >= kStages && !mbar_wait(&kv_empty[stage], phase, abort_flag, p.status, kWaitTimeoutNs, kStatusWaitSite + 41)) break;
           mbar_arrive_expect_tx(&kv_full[stage], 2 * S::kKBytes);
-          bulk_copy(smem + S::kKV + stage * 2 * S::kKBytes, src + static_cast<int64_t>(block_of(j)) * p.hkv * (2 * S::kKBytes),
+          bulk_copy(smem + S::kKV + stage * 2 * S::kKBytes, src + static_cast<int64_t>(all.of(block_of(j))) * p.hkv * (2 * S::kKBytes),
                     2 * S::kKBytes, &kv_full[stage]);
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
@@ -778,7 +795,8 @@ cudaError_t launch(const Params& p, int64_t tiles, cudaStream_t stream) {
   cudaError_t e;
   if (p.tiles != nullptr) {
     if ((e = ensure_smem_attr<kv8_prefill_kernel<D, true>>(Smem<D, true>::kBytes)) != cudaSuccess) return e;
-    e = launch_dependent(kv8_expand_kernel<D>, dim3(p.bt_pages, p.batch, p.hkv), kExpandThreads, 0, stream, p);
+    const unsigned most = static_cast<unsigned>(p.slots_by_tok ? std::min(p.bt_pages, p.slots + p.q_rows / kPage) : p.bt_pages);
+    e = launch_dependent(kv8_expand_kernel<D>, dim3(most, p.batch, p.hkv), kExpandThreads, 0, stream, p);
     if (e != cudaSuccess) return e;
     e = launch_dependent(kv8_prefill_kernel<D, true>, grid, threads(true), Smem<D, true>::kBytes, stream, p);
   } else {
@@ -797,6 +815,22 @@ int64_t row_tiles(int64_t q_rows, int batch, int group, bool expanded) {
   return std::min(q_rows, std::max<int64_t>(0, q_rows - batch) / step + batch);
 }
 
+// Blocks that requests of one batch can see, by what the host knows: a window's span, the sinks and a chunk's own
+// tokens, each with its ragged ends (slots + new / 64 a request), or the whole block table.
+struct Slots {
+  int64_t each, all;
+  bool by_tok;
+  explicit Slots(const Kv8AttnArgs& a) {
+    each = a.window / kPage + 3 + (static_cast<int64_t>(a.sinks) + kPage - 1) / kPage;
+    all = a.batch * each + a.q_rows / kPage + 1;
+    by_tok = a.window > 0 && all < static_cast<int64_t>(a.batch) * a.bt_pages;
+    if (!by_tok) {
+      each = a.bt_pages;
+      all = a.batch * each;
+    }
+  }
+};
+
 }  // namespace
 
 // Bytes of the expanded tiles; 0 where the blocks are expanded in the attention kernel itself.  A launch
@@ -811,7 +845,7 @@ int64_t kv8_prefill_tile_bytes(const Kv8AttnArgs& a) {
   int64_t seen = a.bt_pages;
   if (a.window > 0)
     seen = std::min<int64_t>(seen, (static_cast<int64_t>(a.window) + a.q_rows / std::max(1, a.batch)) / kPage + 2 + (static_cast<int64_t>(a.sinks) + 63) / 64);
-  const int64_t bytes = static_cast<int64_t>(a.batch) * a.bt_pages * a.hkv * kPage * a.head_dim * 4;
+  const int64_t bytes = Slots(a).all * a.hkv * kPage * a.head_dim * 4;
   if (a.q_rows < 4 * step * a.batch || a.q_rows / step * a.hkv * seen < 4200) return 0;
   if (bytes > (int64_t{1} << 31) || a.batch > 65535 || a.hkv > 65535) return 0;
   return bytes;
@@ -864,6 +898,9 @@ cudaError_t kv8_prefill(const Kv8AttnArgs& a, cudaStream_t stream) {
   p.part_o = a.scratch;
   p.part_ml = reinterpret_cast<float2*>(a.scratch + static_cast<int64_t>(a.splits) * a.q_rows * a.hq * a.head_dim);
   p.tiles = static_cast<uint8_t*>(a.tiles);
+  const Slots slots(a);
+  p.slots = static_cast<int>(slots.each);
+  p.slots_by_tok = slots.by_tok ? 1 : 0;
   p.status = a.status;
   const int64_t tiles = row_tiles(a.q_rows, a.batch, group, a.tiles != nullptr) * a.hkv;
   if (tiles > 0x7fffffff) return cudaErrorInvalidValue;

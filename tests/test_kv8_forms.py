@@ -125,3 +125,29 @@ def test_repeats_itself_on_other_streams_and_in_a_graph():
         g.replay()
         torch.cuda.synchronize()
         check_attention(out, q, cache, bt, a, lens, hq, hkv, d, d ** -0.5, 0, 0)
+
+
+def held_beside(f):
+    """f's result and the bytes that it held at most beside what was there."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = f()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - before
+
+
+def test_windows_need_scratch_for_what_they_see():
+    """Wide block tables do not count where a window bounds the blocks (2000 pages of each request would be 1 GB)."""
+    hq, hkv, d, window, sinks = 32, 8, 64, 1024, 70
+    q_lens, kv_lens = [700, 1, 690, 640], [700, 5000, 3000, 1700]
+    pages = sum((n + 63) // 64 for n in kv_lens) + 2
+    cache = make_cache(pages, hkv, d, "cuda", seed=25)
+    bt = make_table(kv_lens, pages, seed=25, width=2000).cuda()
+    assert form(q_lens, bt, hq, hkv, d, window, sinks) == "expanded"
+    q = queries(q_lens, hq, d, 25).cuda()
+    cu, kl = lengths(q_lens, kv_lens)
+    out, held = held_beside(lambda: ops.kv8_prefill_attention(q, cache, bt, cu, kl, hq, hkv, d, window=window, sinks=sinks))
+    assert held < 2 * out.numel() + 24e6
+    check_attention(out, q, cache, bt, q_lens, kv_lens, hq, hkv, d, d ** -0.5, window, sinks)
