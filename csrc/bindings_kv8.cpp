@@ -245,8 +245,12 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& k, cons
   } else {
     torch::Tensor tiles;
     if (const int64_t bytes = omni::kv8_prefill_tile_bytes(a)) {
-      tiles = empty({bytes}, at::kByte, k);
-      a.tiles = tiles.data_ptr();
+      // without the room for them the attention kernel expands the blocks itself
+      try {
+        tiles = empty({bytes}, at::kByte, k);
+        a.tiles = tiles.data_ptr();
+      } catch (const c10::OutOfMemoryError&) {
+      }
     }
     a.splits = omni::kv8_prefill_splits(a, sms);
     if (a.splits > 1) {

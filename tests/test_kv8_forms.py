@@ -151,3 +151,27 @@ def test_windows_need_scratch_for_what_they_see():
     out, held = held_beside(lambda: ops.kv8_prefill_attention(q, cache, bt, cu, kl, hq, hkv, d, window=window, sinks=sinks))
     assert held < 2 * out.numel() + 24e6
     check_attention(out, q, cache, bt, q_lens, kv_lens, hq, hkv, d, d ** -0.5, window, sinks)
+
+
+def test_without_room_for_the_scratch():
+    """Where the expanded blocks find no room, the attention kernel expands them itself."""
+    hq, hkv, d, q_lens, kv_lens = 16, 2, 128, [300, 200], [900, 200]
+    cache = make_cache(25, hkv, d, "cuda", seed=26)
+    bt = make_table(kv_lens, 25, seed=26, width=8000).cuda()              # 1 GB of blocks at most
+    assert form(q_lens, bt, hq, hkv, d) == "expanded"
+    q = queries(q_lens, hq, d, 26).cuda()
+    cu, kl = lengths(q_lens, kv_lens)
+    run = lambda: ops.kv8_prefill_attention(q, cache, bt, cu, kl, hq, hkv, d)  # noqa: E731
+    first, held = held_beside(run)
+    assert held > 1e9
+    del first
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (256 << 20)) / total)
+    try:
+        out, held = held_beside(run)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert held < 256 << 20
+    check_attention(out, q, cache, bt, q_lens, kv_lens, hq, hkv, d, d ** -0.5, 0, 0)
