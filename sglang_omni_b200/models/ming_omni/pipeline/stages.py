@@ -126,14 +126,16 @@ def create_audio_encoder_executor(model_path: str = "", device: str = "cuda:0", 
 
 def create_thinker_executor(model_path: str = "", device: str = "cuda:0", max_batch: int = 64,
                             max_context: int = 8192, max_prefill_tokens: int = 8192, overrides: dict | None = None,
-                            use_graphs: bool = True, thinker_max_seq_len: int | None = None):
+                            use_graphs: bool = True, thinker_max_seq_len: int | None = None,
+                            kv_format: str = "native"):
+    """``kv_format="e4m3"`` keeps the KV cache in 8 bits."""
     dev = torch.device(device)
     model = loader.get_llm(model_path, dev, overrides)
     return qstages.create_thinker_executor(model_path, device, max_batch,
                                            thinker_max_seq_len or max_context, max_prefill_tokens,
                                            overrides=overrides, use_graphs=use_graphs, model=model,
                                            tokenizer=loader.get_tokenizer(model_path, overrides),
-                                           eos_token_ids=loader.eos_ids(model_path, overrides))
+                                           eos_token_ids=loader.eos_ids(model_path, overrides), kv_format=kv_format)
 
 
 # the reference's factory name, so Ming configs written for it resolve
