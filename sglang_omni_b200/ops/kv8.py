@@ -5,7 +5,8 @@ power-of-two exponent (int8) per (token, KV head) row ``[pages, Hkv, 64]``.  A r
 ``rne_e4m3(x * 2^-e)`` with the smallest integer e in [-60, 60] that keeps ``max|x| * 2^-e <= 448``,
 and stands for ``code * 2^e``; values beyond 448 * 2^60 saturate.  A row with an infinity or a NaN is
 marked (exponent -128) and stands for NaN: a query that sees it gets NaN, others are not touched.
-D + 1 bytes a row instead of 2 D.  Head dims 64 and 128, any number of query heads per KV head.
+D + 1 bytes a row instead of 2 D.  Head dims 64 and 128, up to 128 query heads per KV head.  Exponents outside the
+format, which no write leaves, count as the nearest of it.
 
 Attention is causal.  ``window`` > 0 limits a query to its last ``window`` keys plus the request's
 first ``sinks`` tokens.  A query that sees no key (an empty context) gives zeros.

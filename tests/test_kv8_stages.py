@@ -77,3 +77,17 @@ def test_ming_thinker_takes_the_format():
             return last
 
     assert len(asyncio.run(main()).token_ids) == 5
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_example(device):
+    """Codes are off by at most 2^-4 of themselves (2.6 % rms): keys and values each bring that much, 8 % bounds both."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(__file__), "..", "examples", "kv8_cache.py")
+    spec = importlib.util.spec_from_file_location("kv8_cache_example", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    worst, same = example.main(["--device", device, "--prompt", "150", "--chunk", "100", "--steps", "3"])
+    assert 0 < worst < 0.08 and same
