@@ -175,3 +175,22 @@ def test_dependent_launches_behind_a_chunk(new, d):
     for _ in range(3):
         for a, b in zip(layers(lambda: None), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,batch,new,width", [("in place", 33, 21, 30), ("in place", 70, 30, 30), ("expanded", 40, 130, 60)])
+def test_more_requests_than_lanes(name, batch, new, width):
+    """Row tiles are found over more than 32 requests, with empty ones among them and chunks beyond their context."""
+    hq, hkv, d, window, sinks = 64, 2, 64, 500, 3
+    q_lens = [0 if b % 11 == 5 else 1 + (b * 7) % new for b in range(batch)]
+    kv_lens = [max(0, n + (-3 if b % 13 == 2 else (b * 97) % 700)) for b, n in enumerate(q_lens)]
+    if name == "expanded":
+        q_lens, window = [n + new for n in q_lens], 0
+    pages = sum((n + 63) // 64 for n in kv_lens) + 2
+    cache = make_cache(pages, hkv, d, "cuda", seed=12)
+    bt = make_table(kv_lens, pages, seed=12, width=width).cuda()
+    assert ext().kv8_chunk_form(sum(q_lens), batch, width, hq, hkv, d, window, sinks) == name
+    q = queries(sum(q_lens), hq * d, 12, "cuda")
+    cu = i32("cuda", *[sum(q_lens[:i]) for i in range(batch + 1)])
+    out = ops.kv8_prefill_attention(q, cache, bt, cu, i32("cuda", *kv_lens), hq, hkv, d, window=window, sinks=sinks)
+    check_attention(out, q, cache, bt, q_lens, kv_lens, hq, hkv, d, d ** -0.5, window, sinks)
