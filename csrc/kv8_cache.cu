@@ -8,9 +8,11 @@
 //
 // kv8_read: rows by slot, as bf16 (exact).
 //
-// Both are bound by bytes, the write also by its instructions (about 15 an element).  Measured: 8191
-// tokens of 32 + 2 x 4 heads of 128 with norm and M-RoPE 36 us = 4.4 TB/s;
-// 130,000 rows of 2 x 4 heads read in 73 us = 5.5 TB/s (copy: 6.55).
+// Both are bound by bytes; the write waits besides for each token's position, its angles and a barrier, in turn
+// (62 % of issue slots, 40 % of DRAM).  Measured, the write in a graph: 8191 tokens of 32 + 2 x 4 heads of 128 with
+// norm, halves 35 us = 4.6 TB/s, adjacent pairs 35, no rotation or norm 27, halves of 24 dims (partners through
+// shared memory) 81; of 32 + 2 x 8 heads of 64 24, 24, 16, 60.  130,000 rows of 2 x 4 heads of 128 read in 73 us =
+// 5.5 TB/s (copy: 6.55).
 //
 // Reference counterpart: the fp8 KV-cache option of SGLang's token-to-KV pool behind
 // sglang_omni/engines/ar/sglang_backend/server_args_builder.py:10-35 (kv_cache_dtype there).

@@ -29,8 +29,8 @@
 //   q is scaled by a power of two to [2^9, 2^10) before it is rounded to fp16.
 //
 // Measured: 5 requests of 52,000 - 130,000 keys, 32 / 8 heads of 128: 204 - 210 us = 6.4 - 6.6 TB/s
-// (copy: 6.55); 64 slots of about 1150 keys, 32 / 4 heads, out of HBM: 22.7 us = 3.3 TB/s, of which about 8 us
-// are launches, look-ups and joining; 48 windows of 4096 keys, 32 / 8 heads of 64: 45 us = 4.5 TB/s; one
+// (copy: 6.55); 64 slots of about 1150 keys, 32 / 4 heads, out of HBM: 20.7 us = 3.6 TB/s by one CTA a
+// pair, 22.6 over all tiles, of which about 8 us are launches, look-ups and joining; 48 windows of 4096 keys, 32 / 8 heads of 64: 45 us = 4.5 TB/s; one
 // request of 517 keys: 6.3 us.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -753,10 +753,11 @@ int widest_cluster(const Kv8AttnArgs& a) {
 // look-up of the other requests, but its shares follow its own request alone: taken where the pairs
 // with their clusters fit the GPU at once and no share can be long: 24 tiles at what the block table's width and
 // the window allow.  In a graph, 32 / 4 heads of 128, microseconds by all tiles / by clusters: 1 request of
-// 500 keys 7.3 / 5.7, of 8000 (8 CTAs, 16 tiles) 12.8 / 10.7, of 16,000 (31 tiles) 15.1 / 16.5; 16 requests of
-// 2000 (4 CTAs, 8 tiles) 13.3 / 11.2, of 4000 16.5 / 16.1, of 8000 28.0 / 28.6; one CTA a pair, 64 slots of 1280
-// 22.7 / 20.9, of 2000 31.3 / 30.3, of 3000 40.5 / 41.4; nearly a CTA for each pair, 100 slots of 3000 56.8 / 51.2, of
-// 2200 - 4500 64.7 / 64.5.
+// 500 keys 7.2 / 5.8, of 8000 (8 CTAs, 16 tiles) 12.6 / 10.9, of 16,000 (31 tiles) 15.2 / 16.9; 16 requests of
+// 2000 (4 CTAs, 8 tiles) 14.3 / 12.4, of 4000 20.3 / 18.8, of 8000 29.7 / 30.2; one CTA a pair, 64 slots of 1280
+// 22.6 / 21.0, of 2000 31.1 / 30.6, of 3000 40.2 / 41.8; nearly a CTA for each pair, 100 slots of 3000 56.8 / 51.4, of
+// 2200 - 4500 64.7 / 64.5.  A wider table changes neither form's time, only which is taken: 64 slots of 1280 keys in
+// tables of 4096 run over all tiles, 22.6 us; 1 request of 500 in one of 32,768 7.1.
 int kv8_decode_cluster(const Kv8AttnArgs& a) {
   const int64_t pairs = pairs_of(a), tiles = most_tiles(a);
   const int c = widest_cluster(a);
@@ -765,10 +766,12 @@ int kv8_decode_cluster(const Kv8AttnArgs& a) {
 
 // Chunks of few tokens: the decode kernel reads the context once per token (mostly out of L2), the chunk
 // kernel once, but expands it.  Taken where every pair runs at once with at most 16 tiles to a CTA, and for one
-// or two tokens a request.  In a graph, 32 / 4 heads of 128, microseconds by the decode / chunk kernel: one request
-// of 4 tokens on 2000 keys 7.7 / 12.3, on 32,000 24.5 / 26.8; 8 on 8000 16.5 / 18.7, on 16,000 23.5 / 21.5; 16 on 4000
-// 16.7 / 19.1, on 16,000 36 / 24; 96 on 500 12.4 / 23.7, on 4000 48 / 31; 4 requests of 4 on 4000 16.4 / 16.7, on 8000
-// 47 / 23; 16 requests of 2 on 4000 40 / 38, on 32,000 136 / 328.
+// or two tokens a request in the mean (requests without new tokens count; the lengths are on the device).  In a
+// graph, 32 / 4 heads of 128, microseconds by the decode / chunk kernel: one request of 4 tokens on 2000 keys
+// 7.6 / 12.2, on 32,000 26.1 / 27.5; 8 on 8000 17.0 / 18.6, on 16,000 23.9 / 21.4; 16 on 4000 16.9 / 19.1, on 16,000
+// 36 / 24; 96 on 500 12.6 / 16.5, on 4000 50 / 24; 4 requests of 4 on 4000 17.3 / 16.6, on 8000 25.7 / 23.5; 16
+// requests of 2 on 4000 28 / 38, on 32,000 164 / 228.  Uneven batches: 63 requests of one token on 500 keys beside 65
+// tokens on 100,000 905 / 1362, beside 65 on 20,000 159 / 314; 15 beside 17 on 32,000 77 / 228.
 bool kv8_few_tokens(const Kv8AttnArgs& a) {
   const int64_t rows = a.q_rows, requests = a.batch;
   if (rows > 512 || rows * a.bt_pages >= (int64_t{1} << 31)) return false;

@@ -25,9 +25,9 @@
 // outputs are joined in order by a second, dependent launch.  The row tiles are found on the device
 // from cu_q, so a launch depends on sizes alone.
 //
-// Measured, 32 / 4 heads of 128: 2048 new tokens on 32,768 keys 905 us = 1253 TFLOP/s cold, 1047 us when
+// Measured, 32 / 4 heads of 128: 2048 new tokens on 32,768 keys 897 us = 1264 TFLOP/s cold, 1027 us when
 // repeated under the power cap (cuBLAS bf16: 1627 and 1391); 8 chunks of 100 - 1024 tokens on up to 2500
-// keys 172 - 183 us.  The two-tile loop takes about 1600 cycles a block: 1024 of tensor-core arithmetic
+// keys 168 - 178 us.  The two-tile loop takes about 1600 cycles a block: 1024 of tensor-core arithmetic
 // (1280 with the shared-memory reads of 64-key S products), 1024 of exponentials.  Sixteen softmax
 // warps (two threads a row) took 987 us, weights at the last maximum beside the block's own 949, persistent CTAs
 // that fetch the next tile early 949.
@@ -835,11 +835,13 @@ struct Slots {
 
 // Bytes of the expanded tiles; 0 where the blocks are expanded in the attention kernel itself.  A launch
 // of its own costs each block a write and reads of the expanded form, but once for all row tiles of its
-// request: taken from four of them on, where the CTAs have enough blocks to win the launch back: 4200
+// request: taken from four of them on in the mean, where the CTAs have enough blocks to win the launch back: 4200
 // (row tile, KV head, block) triples, 28 on each SM.  In a graph, microseconds with / without it, 32 / 4 heads of 128 (16
-// tokens a row tile): one request of 64 tokens on 16,000 keys (28 an SM) 43 / 38, on 64,000 107 / 113; 96 on 8000 (20)
-// 38 / 34, on 16,000 (40) 50 / 52; 128 on 3000 31 / 25, on 16,000 57 / 69; 1024 on themselves 31 / 28, on 1000 more 46 / 56;
-// four of 32 (two row tiles each) on 8000 50 / 42, of 64 62 / 69.
+// tokens a row tile): one request of 64 tokens on 16,000 keys (28 an SM) 43 / 38, on 64,000 105 / 111; 96 on 8000 (20)
+// 36 / 34, on 16,000 (40) 50 / 51; 128 on 3000 30 / 25, on 16,000 56 / 68; 1024 on themselves 29 / 28, on 1000 more 46 / 55;
+// four of 32 (two row tiles each) on 8000 55 / 43, of 64 66 / 69.  Uneven batches: 2048 tokens on themselves beside 63
+// requests of one token on 500 keys 92 / 101, on 4000 294 / 182; 512 on 2000 beside 15 of one on 500 48 / 39; 2048 on 4000
+// beside 15 of 16 on 500 106 / 184.
 int64_t kv8_prefill_tile_bytes(const Kv8AttnArgs& a) {
   const int64_t step = kRows / (a.hq / a.hkv);
   int64_t seen = a.bt_pages;
